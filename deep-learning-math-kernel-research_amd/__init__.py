@@ -20,11 +20,15 @@ LIB_PATH = os.environ.get("EULER_HIP_LIB") or os.path.join(_HERE, "libeuler_hip.
 
 # ---- enum values of include/euler_hip.h (== the reference's include/euler.hpp) -----------------
 EHIP_OK, EHIP_UNIMPLEMENTED, EHIP_GENERAL_ERROR, EHIP_HIP_ERROR = 0, 1, 2, 3
-F32, F16, U8, S8, S32 = 1, 2, 3, 4, 5
+F32, F16, U8, S8, S32, BF16 = 1, 2, 3, 4, 5, 6
 CONV_AUTO, CONV_DIRECT_1X1, CONV_DIRECT, CONV_WINOGRAD = 0, 1, 2, 4
 NCHW, NHWC, NCHW16C, OIHW, OIHW16I16O, GOIHW = 1, 2, 3, 5, 7, 9
 FINE, COARSE, CALIBRATED = 0, 1, 2
 Q_WEIGHTS_S8, Q_SCALE, Q_SHIFT, Q_WSUM, Q_TINPUT_U8, Q_TOUTPUT_F32 = 1, 2, 3, 4, 5, 6
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU = 0, 1, 2, 3
+ROWS_SORTED, ROWS_TOKEN, ROWS_SLOT = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1
 EL_NO_CALI = float(np.finfo(np.float32).max)
 FLT_MAX = EL_NO_CALI
 
@@ -44,6 +48,26 @@ class ConvDesc(ctypes.Structure):
         "flatting_o", "flatting_t", "sampling_kind")] + [(k, ctypes.c_float) for k in (
         "input_scale", "input_z", "tinput_scale", "tinput_z", "output_scale", "output_z",
         "sum_scale", "sum_z", "relu_lower", "relu_upper")]
+
+
+class LinearDesc(ctypes.Structure):
+    """ehip_linear_desc_t"""
+    _fields_ = [(k, ctypes.c_int32) for k in (
+        "ic", "oc", "experts", "input_type", "output_type", "activation", "gated", "with_bias",
+        "with_residual")] + [("residual_scale", ctypes.c_float)]
+
+
+class NormDesc(ctypes.Structure):
+    """ehip_norm_desc_t"""
+    _fields_ = [(k, ctypes.c_int32) for k in (
+        "cols", "parts", "data_type", "output_type", "post", "pre", "rows_per_gate")] + [(k, ctypes.c_float) for k in (
+            "block_scale", "residual_scale", "post_eps", "pre_eps")]
+
+
+class RouteDesc(ctypes.Structure):
+    """ehip_route_desc_t"""
+    _fields_ = [(k, ctypes.c_int32) for k in (
+        "experts", "topk", "groups", "open_groups", "group_best", "logits_type", "score", "renormalize")] + [("scale", ctypes.c_float)]
 
 
 class EulerHipError(RuntimeError):
@@ -84,6 +108,16 @@ def _load():
     lib.ehip_reorder_nchw_to_blocked.argtypes = [vp, vp, ci, ci, ci, ci, ci, vp]
     lib.ehip_reorder_blocked_to_nchw.argtypes = [vp, vp, ci, ci, ci, ci, ci, vp]
     lib.ehip_reorder_oihw_to_blocked.argtypes = [vp, vp, ci, ci, ci, ci, vp]
+    for kind, desc in (("linear", LinearDesc), ("norm", NormDesc), ("route", RouteDesc)):
+        getattr(lib, "ehip_%s_create" % kind).argtypes = [ctypes.POINTER(desc), ctypes.POINTER(vp)]
+        getattr(lib, "ehip_%s_destroy" % kind).argtypes = [vp]
+        getattr(lib, "ehip_%s_execute" % kind).argtypes = [vp, vp, vp]
+    lib.ehip_linear_execute_experts.argtypes = [vp, vp, vp]
+    lib.ehip_linear_prepare.argtypes = [vp, vp, vp, vp, vp]
+    lib.ehip_linear_kernel_name.argtypes = [vp, ctypes.c_int64]
+    lib.ehip_linear_kernel_name.restype = ctypes.c_char_p
+    lib.ehip_route_plan_ints.argtypes = [vp, ctypes.c_int64]
+    lib.ehip_route_plan_ints.restype = ctypes.c_int64
     return lib
 
 
@@ -94,6 +128,9 @@ EXPORTED_SYMBOLS = (
     "ehip_conv_execute", "ehip_conv_execute_repeat", "ehip_conv_execute_stages", "ehip_conv_query", "ehip_conv_kernel_name", "ehip_quantize_input_u8",
     "ehip_wino_tinput_range", "ehip_wino_tinput_range_noalloc", "ehip_reorder_nchw_to_blocked", "ehip_reorder_blocked_to_nchw",
     "ehip_reorder_oihw_to_blocked", "ehip_ref_conv_f32_range", "ehip_calibrate_output_quant",
+    "ehip_linear_create", "ehip_linear_destroy", "ehip_linear_prepare", "ehip_linear_execute", "ehip_linear_execute_experts",
+    "ehip_linear_kernel_name", "ehip_norm_create", "ehip_norm_destroy", "ehip_norm_execute", "ehip_route_create",
+    "ehip_route_destroy", "ehip_route_plan_ints", "ehip_route_execute",
 )
 
 
@@ -110,7 +147,8 @@ def _check(rc):
 
 _ehip_call.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
     lib.ehip_conv_execute, lib.ehip_quantize_input_u8, lib.ehip_reorder_nchw_to_blocked,
-    lib.ehip_reorder_blocked_to_nchw)), _check)
+    lib.ehip_reorder_blocked_to_nchw, lib.ehip_linear_execute, lib.ehip_linear_execute_experts, lib.ehip_norm_execute,
+    lib.ehip_route_execute)), _check)
 
 
 def _ptr(x):
@@ -199,6 +237,70 @@ class Conv(_ehip_call.ConvBase):
         buf = np.zeros(n.value // np.dtype(dtype).itemsize, dtype)
         _check(lib.ehip_conv_query(self._h, what, ctypes.c_void_p(buf.ctypes.data), ctypes.byref(n)))
         return buf
+
+
+# ---- the layers between convolutions -------------------------------------------------------------------
+def make_linear_desc(ic, oc, experts=1, input_type=BF16, output_type=BF16, activation=ACT_NONE, gated=False, with_bias=False,
+                     with_residual=False, residual_scale=1.0):
+    return LinearDesc(ic, oc, experts, input_type, output_type, activation, int(gated), int(with_bias), int(with_residual),
+                      residual_scale)
+
+
+def make_norm_desc(cols, data_type=BF16, output_type=None, parts=1, post=NORM_NONE, pre=NORM_RMS, rows_per_gate=0, block_scale=1.0,
+                   residual_scale=1.0, post_eps=1e-5, pre_eps=1e-5):
+    return NormDesc(cols, parts, data_type, data_type if output_type is None else output_type, post, pre, rows_per_gate, block_scale,
+                    residual_scale, post_eps, pre_eps)
+
+
+def make_route_desc(experts, topk, logits_type=F32, score=SCORE_SOFTMAX, groups=1, open_groups=1, group_best=1, renormalize=True,
+                    scale=1.0):
+    return RouteDesc(experts, topk, groups, open_groups, group_best, logits_type, score, int(renormalize), scale)
+
+
+class _Layer:
+    """A handle of the C-ABI: ehip_<kind>_create on construction, ehip_<kind>_destroy on close()."""
+
+    def __init__(self, desc):
+        self.desc = desc
+        h = ctypes.c_void_p()
+        _check(getattr(lib, "ehip_%s_create" % self._kind)(ctypes.byref(desc), ctypes.byref(h)))
+        self._h = h.value
+
+    def close(self):
+        if getattr(self, "_h", None) and lib is not None:
+            getattr(lib, "ehip_%s_destroy" % self._kind)(self._h)
+            self._h = None
+
+    __del__ = close
+
+
+class Linear(_Layer, _ehip_call.LinearBase):
+    """A matrix product with bias, activation and residual, of one matrix (``execute``) or of the experts' matrices
+    (``execute_experts``): see ehip_linear_desc_t."""
+    _kind = "linear"
+
+    def prepare(self, weights, bias=None, scale=None, stream=0):
+        _check(lib.ehip_linear_prepare(self._h, _ptr(weights), _ptr(scale), _ptr(bias), ctypes.c_void_p(stream)))
+
+    def kernel_name(self, rows):
+        return lib.ehip_linear_kernel_name(self._h, rows).decode()
+
+
+class Norm(_Layer, _ehip_call.NormBase):
+    """The norm after a block, its gate and residual scale, and the norm before the next block: see ehip_norm_desc_t."""
+    _kind = "norm"
+
+
+class Router(_Layer, _ehip_call.RouterBase):
+    """The experts of each token and the order of their work: see ehip_route_desc_t."""
+    _kind = "route"
+
+    def plan_ints(self, tokens):
+        """int32 values of the plan that execute() fills for so many tokens"""
+        n = lib.ehip_route_plan_ints(self._h, tokens)
+        if n < 0:
+            raise ValueError("tokens out of range: %d" % tokens)
+        return n
 
 
 # quantize_input_u8(dst, src, count, scale, z, stream=0)

@@ -30,6 +30,10 @@ SOURCES = [
     "ehip_wino_whole.hip", "ehip_wino_whole6.hip", "ehip_wino_whole5.hip", "ehip_wino_whole4.hip",
     "ehip_prepare.hip",
     "ehip_harness.hip",
+    "ehip_linear.hip", "ehip_linear_tile.hip",
+    "ehip_norm.hip",
+    "ehip_route.hip",
+    "ehip_layers_api.hip",
     "ehip_api.hip",
     "euler_api.hip",
 ]
@@ -67,6 +71,9 @@ EXTRA_FLAGS = {
     "ehip_fewch.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "ehip_gemm1x1s.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "ehip_gemm1x1w.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16", "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    # a tile kernel's epilogue indexes its accumulators by constants only where it is unrolled whole; m0, which its loads into
+    # LDS set, is a register that the compiler keeps to itself
+    "ehip_linear_tile.hip": ["-mllvm", "-pragma-unroll-threshold=1000000", "-Wno-inline-asm"],
     # and those of the 1x1 kernels with few input channels
     "ehip_gemm.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
 }
@@ -106,7 +113,7 @@ def build(verbose=True, jobs=8, incremental=False):
     subprocess.check_call(cmd)
     # the Python binding's extension module (host code only; the library's addresses are handed to it at run time)
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden", "-Wall",
-           "-I" + sysconfig.get_paths()["include"], os.path.join(CSRC, "ehip_call.cpp"), "-o", os.path.join(HERE, "_ehip_call.so")]
+           "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(ROOT, "include"), os.path.join(CSRC, "ehip_call.cpp"), "-o", os.path.join(HERE, "_ehip_call.so")]
     if verbose:
         print(" ".join(cmd), flush=True)
     procs.append(("ehip_call.cpp", subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT)))

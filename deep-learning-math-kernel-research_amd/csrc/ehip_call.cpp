@@ -7,7 +7,10 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stddef.h>
+#include <string.h>
 #include <structmember.h>
+
+#include "euler_hip.h"
 
 namespace {
 
@@ -15,7 +18,10 @@ typedef int (*execute_t)(void *, void *, const void *, const void *, const void 
 typedef int (*quantize_t)(void *, const void *, size_t, float, float, void *);
 typedef int (*reorder_t)(void *, const void *, int, int, int, int, int, void *);
 
+typedef int (*layer_t)(const void *, const void *, void *);
+
 execute_t g_execute;
+layer_t g_linear, g_experts, g_norm, g_route;
 quantize_t g_quantize;
 reorder_t g_to_blocked, g_to_nchw;
 PyObject *g_raise;      // called with a status that is not zero, raises
@@ -156,6 +162,121 @@ PyGetSetDef conv_getset[] = {{"_h", conv_get_h, conv_set_h, "address of the C ha
                              {nullptr, nullptr, nullptr, nullptr, nullptr}};
 PyTypeObject conv_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
 
+// ---- linear, norm, route: a handle, and an execute that fills the C-ABI's argument structure --------------------
+// kind of each argument by name, in the order of the structure's fields: p = pointer, q = 64-bit integer, i = 32-bit integer,
+// s = the stream.  `at` maps the order of the Python arguments to that of the fields.
+struct Field {
+  const char *name;
+  char kind;
+  size_t offset;
+};
+
+template <int N>
+PyObject *layer_execute(PyObject *self, const char *fn, layer_t f, const Field (&fields)[N], int required, PyObject *const *args, Py_ssize_t nargs,
+                        PyObject *kwnames, char *block)
+{
+  const char *names[N];
+  for (int i = 0; i < N; ++i) names[i] = fields[i].name;
+  PyObject *v[N];
+  if (!arguments(fn, names, required, args, nargs, kwnames, v)) return nullptr;
+  void *stream = nullptr;
+  for (int i = 0; i < N; ++i) {
+    const Field &d = fields[i];
+    if (d.kind == 's') {
+      if (!stream_or_null(v[i], &stream)) return nullptr;
+    } else if (d.kind == 'p') {
+      void *p;
+      if (!pointer_or_null(v[i], &p)) return nullptr;
+      memcpy(block + d.offset, &p, sizeof(p));
+    } else if (v[i]) {
+      PyObject *n = PyNumber_Index(v[i]);
+      if (!n) return nullptr;
+      const long long q = PyLong_AsLongLong(n);
+      int w = 0;
+      const bool ok = d.kind == 'q' ? !PyErr_Occurred() : as_int(n, &w);
+      Py_DECREF(n);
+      if (!ok) return nullptr;
+      if (d.kind == 'q') memcpy(block + d.offset, &q, sizeof(q));
+      else memcpy(block + d.offset, &w, sizeof(w));
+    }
+  }
+  void *h = reinterpret_cast<ConvBase *>(self)->handle;
+  int rc;
+  Py_BEGIN_ALLOW_THREADS
+  rc = f(h, block, stream);
+  Py_END_ALLOW_THREADS
+  return result(rc);
+}
+
+#define F(S, name, kind, field) {name, kind, offsetof(S, field)}
+PyObject *linear_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
+{
+  typedef ehip_linear_args_t S;
+  static const Field fields[] = {F(S, "output", 'p', output_dev), F(S, "input", 'p', input_dev), F(S, "rows", 'q', rows),
+                                 F(S, "input_scale", 'p', input_scale_dev), F(S, "residual", 'p', residual_dev),
+                                 F(S, "output_stride", 'q', output_stride), F(S, "input_stride", 'q', input_stride),
+                                 F(S, "residual_stride", 'q', residual_stride), {"stream", 's', 0}};
+  S block = {};
+  return layer_execute(self, "execute", g_linear, fields, 3, args, nargs, kwnames, reinterpret_cast<char *>(&block));
+}
+PyObject *experts_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
+{
+  typedef ehip_linear_args_t S;
+  static const Field fields[] = {F(S, "output", 'p', output_dev), F(S, "input", 'p', input_dev), F(S, "slots", 'p', slots_dev),
+                                 F(S, "offsets", 'p', offsets_dev), F(S, "rows", 'q', rows), F(S, "topk", 'i', topk),
+                                 F(S, "input_scale", 'p', input_scale_dev), F(S, "input_rows", 'i', input_rows),
+                                 F(S, "output_rows", 'i', output_rows), F(S, "output_stride", 'q', output_stride),
+                                 F(S, "input_stride", 'q', input_stride), {"stream", 's', 0}};
+  S block = {};
+  return layer_execute(self, "execute_experts", g_experts, fields, 6, args, nargs, kwnames, reinterpret_cast<char *>(&block));
+}
+PyObject *norm_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
+{
+  typedef ehip_norm_args_t S;
+  static const Field fields[] = {F(S, "output", 'p', output_dev), F(S, "block", 'p', block_dev), F(S, "rows", 'q', rows),
+                                 F(S, "output_scale", 'p', output_scale_dev), F(S, "sum", 'p', sum_dev), F(S, "residual", 'p', residual_dev),
+                                 F(S, "gate", 'p', gate_dev), F(S, "part_weights", 'p', part_weights_dev),
+                                 F(S, "post_weight", 'p', post_weight_dev), F(S, "post_bias", 'p', post_bias_dev),
+                                 F(S, "pre_weight", 'p', pre_weight_dev), F(S, "pre_bias", 'p', pre_bias_dev),
+                                 F(S, "output_stride", 'q', output_stride), F(S, "sum_stride", 'q', sum_stride),
+                                 F(S, "block_stride", 'q', block_stride), F(S, "residual_stride", 'q', residual_stride),
+                                 F(S, "gate_stride", 'q', gate_stride), {"stream", 's', 0}};
+  S block = {};
+  return layer_execute(self, "execute", g_norm, fields, 3, args, nargs, kwnames, reinterpret_cast<char *>(&block));
+}
+PyObject *route_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
+{
+  typedef ehip_route_args_t S;
+  static const Field fields[] = {F(S, "ids", 'p', ids_dev), F(S, "weights", 'p', weights_dev), F(S, "plan", 'p', plan_dev),
+                                 F(S, "logits", 'p', logits_dev), F(S, "tokens", 'q', tokens), F(S, "bias", 'p', bias_dev),
+                                 F(S, "logits_stride", 'q', logits_stride), {"stream", 's', 0}};
+  S block = {};
+  return layer_execute(self, "execute", g_route, fields, 5, args, nargs, kwnames, reinterpret_cast<char *>(&block));
+}
+#undef F
+
+#define EHIP_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL | METH_KEYWORDS
+PyMethodDef linear_methods[] = {
+    {"execute", EHIP_FAST(linear_execute),
+     "execute(output, input, rows, input_scale=None, residual=None, output_stride=0, input_stride=0, residual_stride=0, stream=0): "
+     "ehip_linear_execute; tensors, device addresses or None, strides in elements (0: rows without a gap), the stream's address"},
+    {"execute_experts", EHIP_FAST(experts_execute),
+     "execute_experts(output, input, slots, offsets, rows, topk, input_scale=None, input_rows=ROWS_SORTED, output_rows=ROWS_SORTED, "
+     "output_stride=0, input_stride=0, stream=0): ehip_linear_execute_experts"},
+    {nullptr, nullptr, 0, nullptr}};
+PyMethodDef norm_methods[] = {
+    {"execute", EHIP_FAST(norm_execute),
+     "execute(output, block, rows, output_scale=None, sum=None, residual=None, gate=None, part_weights=None, post_weight=None, "
+     "post_bias=None, pre_weight=None, pre_bias=None, output_stride=0, sum_stride=0, block_stride=0, residual_stride=0, gate_stride=0, "
+     "stream=0): ehip_norm_execute"},
+    {nullptr, nullptr, 0, nullptr}};
+PyMethodDef route_methods[] = {
+    {"execute", EHIP_FAST(route_execute),
+     "execute(ids, weights, plan, logits, tokens, bias=None, logits_stride=0, stream=0): ehip_route_execute"},
+    {nullptr, nullptr, 0, nullptr}};
+PyTypeObject linear_type = {PyVarObject_HEAD_INIT(nullptr, 0)}, norm_type = {PyVarObject_HEAD_INIT(nullptr, 0)},
+             route_type = {PyVarObject_HEAD_INIT(nullptr, 0)};
+
 // ---- functions -----------------------------------------------------------------------------------
 PyObject *quantize_input_u8(PyObject *, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
 {
@@ -205,22 +326,26 @@ PyObject *reorder_blocked_to_nchw(PyObject *, PyObject *const *args, Py_ssize_t 
   return reorder("reorder_blocked_to_nchw", g_to_nchw, args, nargs, kwnames);
 }
 
-// bind(execute, quantize_input_u8, reorder_nchw_to_blocked, reorder_blocked_to_nchw, raise)
+// bind(execute, quantize_input_u8, reorder_nchw_to_blocked, reorder_blocked_to_nchw, linear_execute, linear_execute_experts,
+// norm_execute, route_execute, raise)
 PyObject *bind(PyObject *, PyObject *args)
 {
-  unsigned long long e, q, b, n;
+  unsigned long long e, q, b, n, l, x, m, t;
   PyObject *r;
-  if (!PyArg_ParseTuple(args, "KKKKO", &e, &q, &b, &n, &r)) return nullptr;
+  if (!PyArg_ParseTuple(args, "KKKKKKKKO", &e, &q, &b, &n, &l, &x, &m, &t, &r)) return nullptr;
   g_execute = reinterpret_cast<execute_t>(e);
   g_quantize = reinterpret_cast<quantize_t>(q);
   g_to_blocked = reinterpret_cast<reorder_t>(b);
   g_to_nchw = reinterpret_cast<reorder_t>(n);
+  g_linear = reinterpret_cast<layer_t>(l);
+  g_experts = reinterpret_cast<layer_t>(x);
+  g_norm = reinterpret_cast<layer_t>(m);
+  g_route = reinterpret_cast<layer_t>(t);
   Py_INCREF(r);
   Py_XSETREF(g_raise, r);
   Py_RETURN_NONE;
 }
 
-#define EHIP_FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(f)), METH_FASTCALL | METH_KEYWORDS
 PyMethodDef methods[] = {
     {"bind", bind, METH_VARARGS, "addresses of the library's functions, and what raises for a status"},
     {"quantize_input_u8", EHIP_FAST(quantize_input_u8), "quantize_input_u8(dst, src, count, scale, z, stream=0)"},
@@ -233,22 +358,32 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ehip_call", nullptr, -1, methods,
 
 PyMODINIT_FUNC PyInit__ehip_call(void)
 {
-  conv_type.tp_name = "_ehip_call.ConvBase";
-  conv_type.tp_basicsize = sizeof(ConvBase);
-  conv_type.tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_BASETYPE;
-  conv_type.tp_new = PyType_GenericNew;
-  conv_type.tp_methods = conv_methods;
-  conv_type.tp_getset = conv_getset;
-  if (PyType_Ready(&conv_type) < 0) return nullptr;
+  const struct {
+    PyTypeObject *type;
+    const char *name;
+    PyMethodDef *methods;
+  } bases[] = {{&conv_type, "_ehip_call.ConvBase", conv_methods}, {&linear_type, "_ehip_call.LinearBase", linear_methods},
+               {&norm_type, "_ehip_call.NormBase", norm_methods}, {&route_type, "_ehip_call.RouterBase", route_methods}};
+  for (const auto &b : bases) {
+    b.type->tp_name = b.name;
+    b.type->tp_basicsize = sizeof(ConvBase);
+    b.type->tp_flags = Py_TPFLAGS_DEFAULT | Py_TPFLAGS_BASETYPE;
+    b.type->tp_new = PyType_GenericNew;
+    b.type->tp_methods = b.methods;
+    b.type->tp_getset = conv_getset;
+    if (PyType_Ready(b.type) < 0) return nullptr;
+  }
   g_data_ptr = PyUnicode_InternFromString("data_ptr");
   if (!g_data_ptr) return nullptr;
   PyObject *m = PyModule_Create(&module);
   if (!m) return nullptr;
-  Py_INCREF(&conv_type);
-  if (PyModule_AddObject(m, "ConvBase", reinterpret_cast<PyObject *>(&conv_type)) < 0) {
-    Py_DECREF(&conv_type);
-    Py_DECREF(m);
-    return nullptr;
+  for (const auto &b : bases) {
+    Py_INCREF(b.type);
+    if (PyModule_AddObject(m, strrchr(b.name, '.') + 1, reinterpret_cast<PyObject *>(b.type)) < 0) {
+      Py_DECREF(b.type);
+      Py_DECREF(m);
+      return nullptr;
+    }
   }
   return m;
 }

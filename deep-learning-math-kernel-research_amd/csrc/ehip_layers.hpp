@@ -1,0 +1,293 @@
+// What the kernels of linear, norm, route and experts share: their arguments, element types, the epilogue of a product.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "euler_hip.h"
+
+namespace ehip {
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+typedef int i4 __attribute__((ext_vector_type(4)));
+typedef int i4u __attribute__((ext_vector_type(4), aligned(1)));   // any address: the load is still one instruction
+typedef __bf16 bf8 __attribute__((ext_vector_type(8)));
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+
+// ---- linear ------------------------------------------------------------------------------------------------------
+// The packed weights are matrix-core operands: 16 rows x 64 bytes of K = 1 KB, lane l holding the 16 bytes of row l % 16
+// from byte 16 * (l / 16) on.  [expert][tile of 16 rows][chunk of 64 bytes][lane].  Four tiles are a group of 64 output
+// columns; row i of tile t in it is column 16 * (i / 4) + 4 * t + i % 4, so that a lane, which holds rows 4 g .. 4 g + 3 of
+// each tile's result, has 16 columns beside each other.  Gated: tiles 0, 2 are the gates of 32 columns, 1, 3 their partners:
+// row i of tiles 2 u, 2 u + 1 is column 8 * (i / 4) + 4 * u + i % 4.
+struct LinearArgs {
+  const char *w;          // packed
+  const float *wscale;    // [expert][tile][16] in the order of the packed rows, or null
+  const float *bias;      // likewise
+  const char *zeros;      // 16 bytes of zeros
+  const char *x;
+  const float *xscale;
+  char *out;
+  const char *res;
+  const int32_t *slots, *offsets;   // experts, or null
+  long long ldx, ldo, ldr;          // bytes
+  long long rows;
+  int oc, kbytes;         // real columns of the output, real bytes of K
+  int tiles, chunks;      // of the packed weights, per expert: a multiple of 4, a multiple of 2
+  int experts, topk, in_rows, out_rows;
+  int out_type, act, gated;
+  float res_scale;
+  int blocks_m, blocks_n;   // set by the launcher
+};
+
+hipError_t launch_linear_pack(void *packed, const void *weights, int experts, int oc, int ic, int elem, int gated, int tiles, int chunks,
+                              char *zeros, hipStream_t s);
+hipError_t launch_linear_constants(float *dst, const float *src, int experts, int oc, int gated, int tiles, hipStream_t s);
+hipError_t launch_linear(const LinearArgs &a, int type, hipStream_t s);
+const char *linear_kernel_name(const LinearArgs &a, int type);
+
+struct NormArgs {
+  char *out;
+  float *out_scale;
+  char *sum;
+  const char *block, *res, *gate;
+  const float *pw, *w1, *b1, *w2, *b2;
+  long long ldo, lds, ldb, ldr, ldg;   // bytes
+  long long rows;
+  int cols, parts, post, pre, rows_per_gate;
+  float block_scale, res_scale, eps1, eps2;
+};
+hipError_t launch_norm(const NormArgs &a, int type, int out_s8, hipStream_t s);
+
+struct RouteArgs {
+  int32_t *ids;
+  float *weights;
+  int32_t *offsets, *slots, *hist;   // hist: [blocks of kRouteBlock tokens][experts]
+  const char *logits;
+  const float *bias;
+  long long tokens, ld;   // ld in bytes
+  int experts, topk, groups, open, best, sigmoid, renorm;
+  float scale;
+};
+constexpr int kRouteBlock = 128;   // tokens of a workgroup
+hipError_t launch_route(const RouteArgs &a, int type, hipStream_t s);
+
+#if defined(__HIPCC__)
+
+__device__ __forceinline__ unsigned pack_bf16(float a, float b)
+{
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  bf2 v = {(__bf16)a, (__bf16)b};
+  return __builtin_bit_cast(unsigned, v);
+}
+__device__ __forceinline__ unsigned pack_f16(float a, float b)
+{
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  h2 v = {(_Float16)a, (_Float16)b};
+  return __builtin_bit_cast(unsigned, v);
+}
+// the two values of a dword
+__device__ __forceinline__ void unpack(unsigned d, bool bf16, float &lo, float &hi)
+{
+  if (bf16) {
+    lo = __builtin_bit_cast(float, d << 16);
+    hi = __builtin_bit_cast(float, d & 0xffff0000u);
+  } else {
+    lo = (float)__builtin_bit_cast(_Float16, (uint16_t)(d & 0xffffu));
+    hi = (float)__builtin_bit_cast(_Float16, (uint16_t)(d >> 16));
+  }
+}
+// one element of type EHIP_F32 / F16 / BF16
+__device__ __forceinline__ float load_one(const char *p, int type)
+{
+  if (type == EHIP_F32) return *reinterpret_cast<const float *>(p);
+  if (type == EHIP_F16) return (float)*reinterpret_cast<const _Float16 *>(p);
+  return (float)*reinterpret_cast<const __bf16 *>(p);
+}
+__device__ __forceinline__ void store_one(char *p, int type, float v)
+{
+  if (type == EHIP_F32) *reinterpret_cast<float *>(p) = v;
+  else if (type == EHIP_F16) *reinterpret_cast<_Float16 *>(p) = (_Float16)v;
+  else *reinterpret_cast<__bf16 *>(p) = (__bf16)v;
+}
+
+// 16 bytes at p of which the first `valid` exist; the others are zero.  ELEM: bytes of an element
+template <int ELEM>
+__device__ __forceinline__ i4 load_part(const char *p, int valid)
+{
+  if (valid >= 16) return *reinterpret_cast<const i4u *>(p);
+  uint64_t half[2] = {0, 0};
+#pragma unroll
+  for (int j = 0; j < 16 / ELEM; ++j)
+    if ((j + 1) * ELEM <= valid) {
+      const uint64_t e = ELEM == 1 ? (uint64_t)reinterpret_cast<const uint8_t *>(p)[j] : (uint64_t)reinterpret_cast<const uint16_t *>(p)[j];
+      half[j * ELEM / 8] |= e << (8 * (j * ELEM % 8));
+    }
+  return i4{(int)half[0], (int)(half[0] >> 32), (int)half[1], (int)(half[1] >> 32)};
+}
+
+// The matrix instruction on two 16-byte operands: 16 rows of weights x 16 rows of activations, 64 bytes of K.  Lane l gets
+// rows 4 * (l / 16) .. + 3 of the weights for row l % 16 of the activations.
+template <int TYPE> struct Product;
+template <> struct Product<EHIP_BF16> {
+  typedef f4 Acc;
+  static constexpr int elem = 2;
+  __device__ static __forceinline__ Acc mma(i4 w, i4 x, Acc c)
+  {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf8, w), __builtin_bit_cast(bf8, x), c, 0, 0, 0);
+  }
+};
+template <> struct Product<EHIP_F16> {
+  typedef f4 Acc;
+  static constexpr int elem = 2;
+  __device__ static __forceinline__ Acc mma(i4 w, i4 x, Acc c)
+  {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, w), __builtin_bit_cast(h8, x), c, 0, 0, 0);
+  }
+};
+template <> struct Product<EHIP_S8> {
+  typedef i4 Acc;
+  static constexpr int elem = 1;
+  __device__ static __forceinline__ Acc mma(i4 w, i4 x, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0); }
+};
+
+__device__ __forceinline__ float activate(float v, int act)
+{
+  if (act == EHIP_ACT_RELU) return v > 0.0f ? v : v != v ? v : 0.0f;
+  if (act == EHIP_ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
+  // the exponential of a large negative v is infinite and the quotient -0, as the limit is
+  if (act == EHIP_ACT_SILU) return v / (1.0f + __expf(-v));
+  return v;
+}
+
+// a tile's sums of one lane as f32: scaled (s8), with bias.  at: the lane's first row in the packed order
+template <typename Acc>
+__device__ __forceinline__ f4 finish_sums(const LinearArgs &a, Acc acc, long long at, float xs)
+{
+  f4 v = {(float)acc[0], (float)acc[1], (float)acc[2], (float)acc[3]};
+  if (a.wscale) {
+    const f4 ws = *reinterpret_cast<const f4 *>(a.wscale + at);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] *= xs * ws[r];
+  }
+  if (a.bias) {
+    const f4 b = *reinterpret_cast<const f4 *>(a.bias + at);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] += b[r];
+  }
+  return v;
+}
+
+// N (a multiple of 4) columns beside each other of one row, from column `col` on: residual, rounding, store.  Columns past the
+// last are dropped.
+template <int N>
+__device__ __forceinline__ void store_columns(const LinearArgs &a, float (&v)[N], char *orow, const char *rrow, int col)
+{
+  const int size = a.out_type == EHIP_F32 ? 4 : 2;
+  const bool bf16 = a.out_type == EHIP_BF16;
+  char *o = orow + (long long)col * size;
+  const char *r = rrow ? rrow + (long long)col * size : nullptr;
+  const int n = a.oc - col;
+  if (n < N) {
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (q < n) store_one(o + q * size, a.out_type, r ? __builtin_fmaf(a.res_scale, load_one(r + q * size, a.out_type), v[q]) : v[q]);
+    return;
+  }
+  if (a.out_type == EHIP_F32) {
+    typedef float fu __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+    for (int q = 0; q < N; q += 4) {
+      fu s = {v[q], v[q + 1], v[q + 2], v[q + 3]};
+      if (r) {
+        const fu old = *reinterpret_cast<const fu *>(r + 4 * q);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[j] = __builtin_fmaf(a.res_scale, old[j], s[j]);
+      }
+      *reinterpret_cast<fu *>(o + 4 * q) = s;
+    }
+    return;
+  }
+  // 4 columns of 16 bits are 8 bytes, 8 are 16
+  constexpr int STEP = N % 8 == 0 ? 8 : 4;
+  typedef unsigned dw __attribute__((ext_vector_type(STEP / 2), aligned(2)));
+#pragma unroll
+  for (int q = 0; q < N; q += STEP) {
+    if (r) {
+      const dw old = *reinterpret_cast<const dw *>(r + 2 * q);
+#pragma unroll
+      for (int j = 0; j < STEP / 2; ++j) {
+        float lo, hi;
+        unpack(old[j], bf16, lo, hi);
+        v[q + 2 * j] = __builtin_fmaf(a.res_scale, lo, v[q + 2 * j]);
+        v[q + 2 * j + 1] = __builtin_fmaf(a.res_scale, hi, v[q + 2 * j + 1]);
+      }
+    }
+    dw p;
+#pragma unroll
+    for (int j = 0; j < STEP / 2; ++j) p[j] = bf16 ? pack_bf16(v[q + 2 * j], v[q + 2 * j + 1]) : pack_f16(v[q + 2 * j], v[q + 2 * j + 1]);
+    *reinterpret_cast<dw *>(o + 2 * q) = p;
+  }
+}
+
+// Rows of the activations and of the output for position `p` of the product.  there = false: a slot that is out of range,
+// whose row 0 may be read in its place and which is not written
+struct RowOf {
+  long long in, out;
+  bool there;
+};
+__device__ __forceinline__ RowOf row_of(const LinearArgs &a, long long p)
+{
+  RowOf r = {p, p, true};
+  if (a.slots && (a.in_rows != EHIP_ROWS_SORTED || a.out_rows != EHIP_ROWS_SORTED)) {
+    const int s = a.slots[p];
+    r.there = s >= 0 && s < a.rows;
+    const int c = r.there ? s : 0;
+    if (a.in_rows != EHIP_ROWS_SORTED) r.in = a.in_rows == EHIP_ROWS_TOKEN ? c / a.topk : c;
+    if (a.out_rows != EHIP_ROWS_SORTED) r.out = c;
+  }
+  return r;
+}
+
+// Which expert's positions [first, last) the index-th block of `rows` of them has, blocks counted expert after expert; past
+// the last one there is no work (expert < 0).  Every lane gets the same answer.  An offset out of range counts as the nearest
+// one in it.
+struct Block {
+  int expert;
+  long long first, last;
+};
+__device__ __forceinline__ Block block_of(const LinearArgs &a, int index, int rows)
+{
+  if (!a.offsets) return {0, (long long)index * rows, a.rows};
+  const int lane = threadIdx.x & 63, most = (int)a.rows;
+  int before = 0;
+  for (int e0 = 0; e0 < a.experts; e0 += 64) {
+    const int e = e0 + lane;
+    int lo = 0, hi = 0;
+    if (e < a.experts) {
+      lo = a.offsets[e];
+      hi = a.offsets[e + 1];
+    }
+    lo = lo < 0 ? 0 : lo > most ? most : lo;
+    hi = hi < lo ? lo : hi > most ? most : hi;
+    const int n = (hi - lo + rows - 1) / rows;
+    int sum = n;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int t = __shfl_up(sum, d);
+      if (lane >= d) sum += t;
+    }
+    const int at = index - before - (sum - n);
+    const unsigned long long who = __ballot(at >= 0 && at < n);
+    if (who) {
+      const int l = __builtin_ctzll(who);
+      return {__builtin_amdgcn_readfirstlane(e0 + l), (long long)__builtin_amdgcn_readlane(lo, l) + (long long)__builtin_amdgcn_readlane(at, l) * rows,
+              __builtin_amdgcn_readlane(hi, l)};
+    }
+    before += __builtin_amdgcn_readlane(sum, 63);
+  }
+  return {-1, 0, 0};
+}
+
+#endif
+}  // namespace ehip

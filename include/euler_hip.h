@@ -29,6 +29,7 @@ enum { EHIP_OK = 0, EHIP_UNIMPLEMENTED = 1, EHIP_GENERAL_ERROR = 2, EHIP_HIP_ERR
 
 /* data types (include/euler.hpp:66-73) */
 enum { EHIP_DT_UNDEF = 0, EHIP_F32 = 1, EHIP_F16 = 2, EHIP_U8 = 3, EHIP_S8 = 4, EHIP_S32 = 5 };
+enum { EHIP_BF16 = 6 };   /* the layers between convolutions only */
 
 /* algorithms (include/euler.hpp:35-42) */
 enum { EHIP_CONV_AUTO = 0, EHIP_CONV_DIRECT_1X1 = 1, EHIP_CONV_DIRECT = 2, EHIP_CONV_WINOGRAD = 4 };
@@ -203,6 +204,125 @@ EHIP_API int ehip_reorder_blocked_to_nchw(void *dst_dev, const void *src_dev, in
                                           int c, int h, int w, void *hip_stream);
 EHIP_API int ehip_reorder_oihw_to_blocked(void *dst_dev, const void *src_dev, int o, int i, int h,
                                           int w, void *hip_stream);
+
+/* ---- the layers between convolutions: linear, norm, route, experts --------------------------------------------------
+ * No counterpart in the reference.  Activations are rows of features, row-major; a stride is the distance of two rows
+ * in elements, 0 meaning rows without a gap.  Addresses need the alignment of their elements only.  No rows is a call
+ * that does nothing.  Handles hold constants (packed weights) and nothing of a call: executes of one handle may overlap
+ * on several streams, and every call can be captured into a graph. */
+
+/* activation functions: erf form of GELU; silu(x) = x / (1 + exp(-x)) */
+enum { EHIP_ACT_NONE = 0, EHIP_ACT_RELU = 1, EHIP_ACT_GELU = 2, EHIP_ACT_SILU = 3 };
+/* which row of a tensor belongs to position p of the expert order: p itself, the token slots[p] / topk, the slot slots[p] */
+enum { EHIP_ROWS_SORTED = 0, EHIP_ROWS_TOKEN = 1, EHIP_ROWS_SLOT = 2 };
+enum { EHIP_NORM_NONE = 0, EHIP_NORM_RMS = 1, EHIP_NORM_LAYER = 2 };
+enum { EHIP_SCORE_SOFTMAX = 0, EHIP_SCORE_SIGMOID = 1 };
+
+/* output[m][o] = act(a[m][o]) + residual_scale * residual[m][o],   a[m][o] = sum_i input[m][i] * weights[o][i] + bias[o];
+ * gated: weights and bias hold 2 * oc rows, first those of the gates, and the output is act(a[m][o]) * a[m][oc + o].
+ * input_type EHIP_F16 / EHIP_BF16 (weights alike, sums in f32) or EHIP_S8: codes with one scale per input row and one per
+ * weights row, sums in s32.  output_type EHIP_F32 / EHIP_F16 / EHIP_BF16, also the residual's; rounded once, at the end.
+ * experts > 1: one matrix per expert, for ehip_linear_execute_experts. */
+typedef struct ehip_linear_desc {
+  int32_t ic, oc, experts;
+  int32_t input_type, output_type;
+  int32_t activation, gated, with_bias, with_residual;
+  float residual_scale;
+} ehip_linear_desc_t;
+
+typedef struct ehip_linear_args {
+  void *output_dev;
+  const void *input_dev;
+  const float *input_scale_dev;      /* s8: one per input row                                                  */
+  const void *residual_dev;          /* with_residual; may be the output itself (same address and stride)      */
+  const int32_t *slots_dev;          /* experts: [rows] slot (token * topk + choice) at each position           */
+  const int32_t *offsets_dev;        /* experts: [experts + 1] first position of each expert's, ascending       */
+  int64_t rows;                      /* rows of the product; experts: slots, i.e. tokens * topk                 */
+  int64_t output_stride, input_stride, residual_stride;
+  int32_t topk, input_rows, output_rows;   /* experts: EHIP_ROWS_*                                             */
+} ehip_linear_args_t;
+
+typedef struct ehip_linear ehip_linear_t;
+
+/* Validates the descriptor and allocates the packed weights.  Limits: ic and oc up to 2^24, experts up to 1024; s8: ic
+ * up to 131071 (the s32 sum cannot overflow). */
+EHIP_API int ehip_linear_create(const ehip_linear_desc_t *desc, ehip_linear_t **out);
+EHIP_API int ehip_linear_destroy(ehip_linear_t *linear);
+/* Packs weights [experts][oc (gated: 2 oc)][ic], and keeps copies of scale (s8) and bias, f32 [experts][oc or 2 oc].
+ * Asynchronous on `hip_stream`; executes on other streams have to be ordered behind it by the caller. */
+EHIP_API int ehip_linear_prepare(ehip_linear_t *linear, const void *weights_dev, const float *scale_dev, const float *bias_dev,
+                                 void *hip_stream);
+EHIP_API int ehip_linear_execute(const ehip_linear_t *linear, const ehip_linear_args_t *args, void *hip_stream);
+/* The product of every position p in [offsets[e], offsets[e + 1]) with the matrix of expert e; no residual.  Output rows
+ * that no position leads to are left as they are.  A slot outside [0, rows) is skipped. */
+EHIP_API int ehip_linear_execute_experts(const ehip_linear_t *linear, const ehip_linear_args_t *args, void *hip_stream);
+/* Name of the kernel that a call with so many rows runs. */
+EHIP_API const char *ehip_linear_kernel_name(const ehip_linear_t *linear, int64_t rows);
+
+/* The norm after a block, its gate and residual scale, and the norm before the next block, in one pass over the rows:
+ *   y = block[r]   (parts > 1: sum over j of part_weights[r][j] * block[r * parts + j]; a part of weight 0 is not read)
+ *   h = residual_scale * residual[r] + block_scale * gate[r / rows_per_gate] * post(y)
+ *   sum[r] = h,  output[r] = pre(h)
+ * RMS: x / sqrt(mean(x^2) + eps) * weight + bias, LAYER: the same of x - mean(x).  Weights and biases f32, null = 1 and 0.
+ * data_type EHIP_F32 / F16 / BF16: block, residual, gate, sum and output; output_type EHIP_S8 instead: codes, and
+ * output_scale[r] = max |pre(h)| / 127.  Everything between is f32; pre() sees h before it is rounded. */
+typedef struct ehip_norm_desc {
+  int32_t cols, parts;
+  int32_t data_type, output_type;
+  int32_t post, pre;                 /* EHIP_NORM_*                                                            */
+  int32_t rows_per_gate;             /* 0: one gate row for all                                                */
+  float block_scale, residual_scale, post_eps, pre_eps;
+} ehip_norm_desc_t;
+
+typedef struct ehip_norm_args {
+  void *output_dev;                  /* may be the block itself (parts = 1, same type and stride), or null      */
+  float *output_scale_dev;           /* s8 output                                                              */
+  void *sum_dev;                     /* null: not wanted; may be the residual itself (same stride)             */
+  const void *block_dev, *residual_dev /* or null */, *gate_dev /* or null */;
+  const float *part_weights_dev;     /* [rows][parts], with parts > 1                                          */
+  const float *post_weight_dev, *post_bias_dev, *pre_weight_dev, *pre_bias_dev;
+  int64_t rows;
+  int64_t output_stride, sum_stride, block_stride, residual_stride, gate_stride;
+} ehip_norm_args_t;
+
+typedef struct ehip_norm ehip_norm_t;
+
+/* cols up to 65536, parts up to 64. */
+EHIP_API int ehip_norm_create(const ehip_norm_desc_t *desc, ehip_norm_t **out);
+EHIP_API int ehip_norm_destroy(ehip_norm_t *norm);
+EHIP_API int ehip_norm_execute(const ehip_norm_t *norm, const ehip_norm_args_t *args, void *hip_stream);
+
+/* The experts of each token and the order of their work.  score = softmax or sigmoid of the token's logits, key = score +
+ * bias.  groups > 1: only the experts of the open_groups groups with the largest sum of their group_best largest keys
+ * stay.  The topk largest keys are chosen, ties going to the lowest index, in groups as well.
+ * ids[t][j] = j-th choice; weights[t][j] = its score, with renormalize divided by the sum over the choices, times scale.
+ * A logit of -inf or NaN (or a key of -inf or NaN) closes its expert to the token; +inf counts as the largest finite
+ * value.  A token with fewer open experts than topk gets id -1 and weight 0 behind them.
+ * The plan holds offsets[experts + 1], the first position of each expert's slots, and from plan[experts + 1] on
+ * slots[tokens * topk]: the slots (token * topk + j) by expert, ascending within one; behind offsets[experts], -1. */
+typedef struct ehip_route_desc {
+  int32_t experts, topk, groups, open_groups, group_best;
+  int32_t logits_type, score, renormalize;
+  float scale;
+} ehip_route_desc_t;
+
+typedef struct ehip_route_args {
+  int32_t *ids_dev;                  /* [tokens][topk] */
+  float *weights_dev;                /* [tokens][topk] */
+  int32_t *plan_dev;                 /* ehip_route_plan_ints(route, tokens) values; null: only ids and weights */
+  const void *logits_dev;
+  const float *bias_dev;             /* [experts] or null */
+  int64_t tokens, logits_stride;
+} ehip_route_args_t;
+
+typedef struct ehip_route ehip_route_t;
+
+/* experts up to 1024, topk up to 32, groups up to 64, tokens * topk below 2^30. */
+EHIP_API int ehip_route_create(const ehip_route_desc_t *desc, ehip_route_t **out);
+EHIP_API int ehip_route_destroy(ehip_route_t *route);
+/* int32 values of a plan for so many tokens (offsets, slots, and what the call keeps while it runs); -1 = bad argument */
+EHIP_API int64_t ehip_route_plan_ints(const ehip_route_t *route, int64_t tokens);
+EHIP_API int ehip_route_execute(const ehip_route_t *route, const ehip_route_args_t *args, void *hip_stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,245 @@
+"""Linear and the experts' products on the GPU against 64 bits: every kernel, type and epilogue at the sizes where a tile, a
+chunk of K or a vector ends, rows with gaps, any alignment.  What lies around the tensors is NaN or a mark, so that a read or a
+write past an edge shows."""
+import math
+
+import pytest
+import torch
+
+import layer_refs as ref
+from layer_refs import E, TORCH
+
+pytestmark = pytest.mark.gpu
+
+# rows x inputs x outputs: one of everything; the last chunk of K whole, ragged by a 16-byte part and by an element; the last
+# column alone; both sides of the row counts at which another kernel takes over
+SIZES = [(1, 1, 1), (1, 64, 64), (2, 33, 17), (15, 200, 31), (16, 512, 130), (17, 63, 65), (32, 520, 64), (33, 129, 33), (64, 1000, 200),
+         (65, 257, 40), (129, 96, 300), (193, 64, 257), (257, 328, 70), (300, 129, 513), (515, 640, 1000)]
+TYPES = [E.BF16, E.F16, E.S8]
+
+
+def rows(g, m, n, dtype, gap, shift, scale=1.0):
+    """m rows of n values in a buffer that is NaN (8 bits: 99) elsewhere: `gap` values between rows, from element `shift` on"""
+    if dtype == torch.int8:
+        v = torch.randint(-127, 128, (m, n), generator=g, device="cuda").to(torch.int8)
+    else:
+        v = (torch.randn((m, n), generator=g, device="cuda") * scale).to(dtype)
+    room = torch.full((shift + m * (n + gap) + 64,), 99 if dtype == torch.int8 else math.nan, dtype=dtype, device="cuda")
+    t = room[shift:shift + m * (n + gap)].view(m, n + gap)[:, :n]
+    t.copy_(v)
+    return t, room
+
+
+class Case:
+    def __init__(self, m, ic, oc, itype, otype, activation=E.ACT_NONE, gated=False, bias=False, residual=False, experts=1, gap=0, shift=0,
+                 seed=0, in_rows=None):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed * 1000003 + m * 10007 + ic * 101 + oc)
+        self.d = E.make_linear_desc(ic, oc, experts=experts, input_type=itype, output_type=otype, activation=activation, gated=gated,
+                                    with_bias=bias, with_residual=residual, residual_scale=0.5)
+        n2 = oc * (2 if gated else 1)
+        self.m, self.gap, self.shift, self.otype = m, gap, shift, TORCH[otype]
+        n_in = m if in_rows is None else in_rows
+        self.x, self.x_room = rows(g, n_in, ic, TORCH[itype], gap, shift)
+        self.w, _ = rows(g, experts * n2, ic, TORCH[itype], 0, 0, ic ** -0.5)
+        self.xs = self.ws = self.b = self.r = None
+        if itype == E.S8:
+            self.xs = torch.rand(n_in, generator=g, device="cuda") / 64
+            self.ws = torch.rand(experts * n2, generator=g, device="cuda") / 64 * ic ** -0.5
+        if bias:
+            self.b = torch.randn(experts * n2, generator=g, device="cuda")
+        if residual:
+            self.r, _ = rows(g, m, oc, self.otype, gap, shift)
+        self.out, self.out_room = rows(g, m, oc, self.otype, gap, shift)
+        self.out_room.fill_(-77)
+        self.h = E.Linear(self.d)
+        self.h.prepare(self.w, bias=self.b, scale=self.ws)
+
+    def run(self, out=None, stream=0):
+        self.h.execute(self.out if out is None else out, self.x, self.m, input_scale=self.xs, residual=self.r,
+                       output_stride=self.out.stride(0) if self.m > 1 else 0, input_stride=self.x.stride(0) if self.m > 1 else 0,
+                       residual_stride=0 if self.r is None or self.m == 1 else self.r.stride(0), stream=stream)
+
+    def check(self):
+        torch.cuda.synchronize()
+        ref.close(self.out, *ref.linear(self.x, self.w, self.d, self.b, self.xs, self.ws, self.r))
+        self.out.fill_(-77)
+        assert (self.out_room == -77).all(), "written outside of the output"
+
+
+@pytest.mark.parametrize("itype", TYPES)
+@pytest.mark.parametrize("m, ic, oc", SIZES)
+def test_product(m, ic, oc, itype):
+    c = Case(m, ic, oc, itype, E.F32)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("itype, otype", [(E.BF16, E.BF16), (E.BF16, E.F16), (E.F16, E.F16), (E.S8, E.BF16), (E.S8, E.F16)])
+@pytest.mark.parametrize("m, ic, oc", SIZES[2:])
+def test_rows_with_gaps_at_any_address(m, ic, oc, itype, otype):
+    c = Case(m, ic, oc, itype, otype, bias=True, residual=True, gap=5, shift=3)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("activation", [E.ACT_NONE, E.ACT_RELU, E.ACT_GELU, E.ACT_SILU])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m, ic, oc", [(1, 96, 35), (20, 200, 64), (50, 130, 129), (200, 96, 35), (260, 264, 300)])
+def test_epilogues(m, ic, oc, gated, activation):
+    for itype, otype, bias, residual in ((E.BF16, E.F32, True, True), (E.S8, E.BF16, True, False), (E.F16, E.F16, False, True)):
+        c = Case(m, ic, oc, itype, otype, activation=activation, gated=gated, bias=bias, residual=residual, gap=3)
+        c.run()
+        c.check()
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_residual_in_place(m):
+    c = Case(m, 192, 100, E.BF16, E.BF16, residual=True, gap=4)
+    c.out.copy_(c.r)
+    before = c.out.clone()
+    c.h.execute(c.out, c.x, m, residual=c.out, output_stride=104, input_stride=196, residual_stride=104)
+    ref.close(c.out, *ref.linear(c.x, c.w, c.d, residual=before))
+
+
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_infinities_and_nan_stay_in_their_rows(m):
+    c = Case(m, 100, 48, E.BF16, E.F32)
+    c.x[0, 5] = math.nan
+    c.x[m - 1, 99] = math.inf
+    c.run()
+    torch.cuda.synchronize()
+    assert torch.isnan(c.out[0]).all()
+    assert (torch.isinf(c.out[m - 1]) | torch.isnan(c.out[m - 1]) | (c.w[:, 99] == 0)).all()
+    ref.close(c.out[1:m - 1], *ref.linear(c.x[1:m - 1], c.w, c.d))
+
+
+def test_no_rows_is_no_call():
+    c = Case(1, 8, 8, E.BF16, E.BF16)
+    c.h.execute(None, None, 0)
+    assert (c.out_room == -77).all()
+
+
+@pytest.mark.parametrize("m", [20, 300])
+def test_rows_past_32_bits(m):
+    """the last rows start more than 2^32 bytes behind the first"""
+    ic, oc, stride = 64, 40, (1 << 32) // (m - 10) // 2 + 8
+    d = E.make_linear_desc(ic, oc)
+    x = torch.zeros(m * stride, dtype=torch.bfloat16, device="cuda").view(m, stride)
+    out = torch.zeros(m * stride, dtype=torch.bfloat16, device="cuda").view(m, stride)
+    x[:, :ic] = torch.randn(m, ic, device="cuda")
+    w = torch.randn(oc, ic, device="cuda").bfloat16()
+    h = E.Linear(d)
+    h.prepare(w)
+    h.execute(out, x, m, output_stride=stride, input_stride=stride)
+    ref.close(out[:, :oc], *ref.linear(x[:, :ic], w, d))
+
+
+def test_streams_and_graph():
+    """executes of one handle on two streams at once, and a captured one replayed on new inputs"""
+    cases = [Case(m, 256, 192, E.BF16, E.BF16, bias=True, activation=E.ACT_SILU, gated=True, seed=s) for s, m in enumerate((5, 48, 400))]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for c in cases:
+        outs = [torch.empty_like(c.out) for _ in streams]
+        for _ in range(8):
+            for s, o in zip(streams, outs):
+                c.run(out=o, stream=s.cuda_stream)
+        c.run()
+        torch.cuda.synchronize()
+        for o in outs:
+            assert torch.equal(o.view(torch.int16), c.out.contiguous().view(torch.int16))
+        c.check()
+    for c in cases:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            c.run(stream=torch.cuda.current_stream().cuda_stream)
+        for i in range(3):
+            c.x.copy_(torch.randn_like(c.x.float()).to(c.x.dtype))
+            g.replay()
+            c.check()
+
+
+def plan(g, tokens, experts, topk, empty=(), dropped=0):
+    """ids of a routing, its slots in expert order (-1 behind the last) and offsets"""
+    ids = torch.stack([torch.randperm(experts, generator=g)[:topk] for _ in range(tokens)]).reshape(-1)
+    ids = torch.where(torch.tensor([int(i) in empty for i in ids]), torch.tensor(-1), ids)
+    ids[:dropped] = -1
+    key = torch.where(ids < 0, experts, ids)
+    order = key.argsort(stable=True)
+    live = int((ids >= 0).sum())
+    slots = order.clone()
+    slots[live:] = -1
+    offsets = torch.searchsorted(key[order], torch.arange(experts + 1))
+    return slots.int().cuda(), offsets.int().cuda(), ids
+
+
+@pytest.mark.parametrize("itype", TYPES)
+@pytest.mark.parametrize("tokens, experts, topk, ic, oc", [(1, 4, 2, 64, 40), (16, 8, 3, 200, 65), (50, 3, 2, 129, 100), (400, 70, 4, 96, 48),
+                                                           (700, 3, 2, 264, 130), (600, 2, 1, 100, 70)])
+@pytest.mark.parametrize("side", ["up", "down"])
+def test_experts(tokens, experts, topk, ic, oc, itype, side):
+    g = torch.Generator()
+    g.manual_seed(tokens)
+    slots, offsets, _ = plan(g, tokens, experts, topk, empty=(1,), dropped=topk)
+    count = tokens * topk
+    up = side == "up"
+    c = Case(count, ic, oc, itype, E.BF16 if itype != E.F16 else E.F16, activation=E.ACT_SILU if up else E.ACT_NONE, gated=up, bias=True,
+             experts=experts, in_rows=tokens if up else count, gap=3)
+    c.h.execute_experts(c.out, c.x, slots, offsets, count, topk, input_scale=c.xs, input_rows=E.ROWS_TOKEN if up else E.ROWS_SORTED,
+                        output_rows=E.ROWS_SORTED if up else E.ROWS_SLOT, output_stride=c.out.stride(0), input_stride=c.x.stride(0))
+    torch.cuda.synchronize()
+    n2, ends = c.w.shape[0] // experts, offsets.tolist()
+    for e in range(experts):
+        p = torch.arange(ends[e], ends[e + 1], device="cuda")
+        if not len(p):
+            continue
+        s = slots[p].long()
+        x = s // topk if up else p
+        o = p if up else s
+        part = slice(e * n2, (e + 1) * n2)
+        ref.close(c.out[o], *ref.linear(c.x[x], c.w[part], c.d, c.b[part], None if c.xs is None else c.xs[x], None if c.ws is None else c.ws[part]))
+        c.out[o] = -77
+    assert (c.out_room == -77).all(), "a row was written that no position leads to"
+
+
+def test_experts_with_slots_out_of_range():
+    """slots and offsets come from memory: what is out of range is neither read nor written"""
+    experts, tokens, topk, ic, oc = 3, 8, 2, 64, 48
+    c = Case(16, ic, oc, E.BF16, E.BF16, experts=experts)
+    slots = torch.arange(16, dtype=torch.int32, device="cuda")
+    slots[2], slots[7] = -5, 1 << 30
+    offsets = torch.tensor([-4, 6, 3, 1 << 20], dtype=torch.int32, device="cuda")
+    c.h.execute_experts(c.out, c.x, slots, offsets, 16, topk, input_rows=E.ROWS_SLOT, output_rows=E.ROWS_SLOT)
+    torch.cuda.synchronize()
+    assert (c.out[2] == -77).all() and (c.out[7] == -77).all()
+    ref.close(c.out[:2], *ref.linear(c.x[:2], c.w[:oc], c.d))
+    ref.close(c.out[8:], *ref.linear(c.x[8:], c.w[2 * oc:], c.d))
+    c.out.fill_(-77)
+    assert (c.out_room == -77).all()
+
+
+def test_calls_are_checked_before_a_launch():
+    h = E.Linear(E.make_linear_desc(64, 32, input_type=E.S8, with_bias=True, with_residual=True))
+    with pytest.raises(E.EulerHipError, match="not prepared"):
+        h.execute(256, 256, 4)
+    w, s = torch.zeros((32, 64), dtype=torch.int8, device="cuda"), torch.zeros(32, device="cuda")
+    for kw, match in (({"bias": s}, "scale per row"), ({"scale": s}, "no bias"), ({"scale": s.data_ptr() + 2, "bias": s}, "multiple")):
+        with pytest.raises(E.EulerHipError, match=match):
+            h.prepare(w, **kw)
+    h.prepare(w, scale=s, bias=s)
+    for args, kw, match in (((256, 256, 4), {"input_scale": 256}, "null"), ((256, 256, 4), {"residual": 256}, "null"),
+                            ((256, 256, -1), {}, "rows"), ((256, 256, 1 << 31), {}, "rows"), ((256, 256, 4), {"input_stride": 63}, "stride"),
+                            ((257, 256, 4), {"input_scale": 256, "residual": 256}, "multiple")):
+        with pytest.raises(E.EulerHipError, match=match):
+            h.execute(*args, **kw)
+    h = E.Linear(E.make_linear_desc(64, 32, experts=2))
+    h.prepare(torch.zeros((2, 32, 64), dtype=torch.bfloat16, device="cuda"))
+    with pytest.raises(E.EulerHipError, match="offsets"):
+        h.execute(256, 256, 4)
+    for args, kw, match in (((256, 256, 256, 256, 5, 2), {}, "topk"), ((256, 256, 256, 256, 4, 0), {}, "topk"), ((256, 256, None, 256, 4, 2), {}, "null"),
+                            ((256, 256, 256, 256, 4, 2), {"input_rows": 3}, "input rows"), ((256, 256, 256, 256, 4, 2), {"output_rows": 1}, "output rows"),
+                            ((256, 256, 256, 256, 1 << 30, 2), {}, "2\\^30"), ((256, 256, 258, 256, 4, 2), {}, "multiple")):
+        with pytest.raises(E.EulerHipError, match=match):
+            h.execute_experts(*args, **kw)
+    torch.cuda.synchronize()
