@@ -8,12 +8,15 @@ namespace ehip {
 // 64 lanes x 16 bytes from memory into LDS at lds + 16 * lane, no registers between.  The wait is the caller's.
 __device__ __forceinline__ void load_to_lds(const char *src, unsigned lds)
 {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "m0");
 }
 
-// A workgroup has WN x WM waves of NTW x MTW tiles of 16 x 16 results.  A step is 128 bytes of K: while the waves multiply the
-// operands of one step out of LDS, those of the next arrive in the other half.  ALIGNED: rows of activations at multiples of 16
-// bytes and a whole number of 16-byte parts in K, so they go straight into LDS too; else through registers.
+// A workgroup has WN x WM waves of NTW x MTW tiles of 16 x 16 results.  A step is 128 bytes of K, in two halves; LDS holds two
+// steps.  A wave multiplies one half out of registers while it reads the next into others.  The workgroup meets once a step,
+// between the halves: by then every wave has read the whole step, and the next one has arrived; the one after it is loaded
+// into the place that came free.
+// ALIGNED: rows of activations at multiples of 16 bytes and a whole number of 16-byte parts in K, so they go straight into LDS
+// like the weights; else through registers.
 template <int TYPE, int NTW, int MTW, int WN, int WM, bool ALIGNED>
 __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
 {
@@ -43,106 +46,174 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
     const int tile = bn * BN + wave * WL + i;
     wsrc[i] = a.w + ((long long)blk.expert * a.tiles + (tile < a.tiles ? tile : a.tiles - 1)) * a.chunks * 1024 + lane * 16;
   }
-  const char *xsrc[XL];
+  // 8 lanes have the 128 bytes of a row, so that a load is whole lines; the 16-byte parts of row r change places by r % 8, so that
+  // the 8 rows that are read at a time lie in different banks
+  const int part = (lane & 7) ^ (lane >> 3);
+  const char *xsrc[2 * XL];
 #pragma unroll
-  for (int i = 0; i < XL; ++i) {
-    const long long p = blk.first + (wave * XL + i) * 16 + c;
-    xsrc[i] = a.x + row_of(a, p < blk.last ? p : blk.last - 1).in * a.ldx + g * 16;
+  for (int i = 0; i < 2 * XL; ++i) {
+    const long long p = blk.first + (wave * XL * 2 + i) * 8 + (lane >> 3);
+    xsrc[i] = a.x + row_of(a, p < blk.last ? p : blk.last - 1).in * a.ldx + part * 16;
   }
   const unsigned base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
   const int steps = a.chunks >> 1;
+  const int wn = wave % WN, wm = wave / WN;
+  const char *wlds = lds + wn * NTW * 2048 + lane * 16, *xlds = lds + (BN + wm * MTW) * 2048 + c * 128;
+  const int xpart = (g ^ (c & 7)) * 16;   // (of the second half: the same, 64 bytes away)
 
-  i4 xr[XL][2];
-  auto load = [&](int step, int stage) {
-    const unsigned to = base + stage * STAGE;
+  // the j-th of the wave's loads of a step
+  constexpr int LOADS = ALIGNED ? 2 * (WL + XL) : 2 * WL;
+  auto load = [&](int j, int step, int stage) {
+    const int i = j >> 1, h = j & 1;
+    const unsigned to = base + stage * STAGE + h * 1024;
+    if (i < WL) {
+      load_to_lds(wsrc[i < WL ? i : 0] + (long long)step * 2048 + h * 1024, to + (wave * WL + i) * 2048);
+    } else {
+      const int x = j - 2 * WL, at = step * 128;
+      load_to_lds(at + part * 16 < a.kbytes ? xsrc[x < 2 * XL ? x : 0] + at : a.zeros, base + stage * STAGE + (BN + wave * XL) * 2048 + x * 1024);
+    }
+  };
+  i4 xr[2 * XL];
+  auto fetch = [&](int step) {
+    if constexpr (!ALIGNED) {
 #pragma unroll
-    for (int i = 0; i < WL; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) load_to_lds(wsrc[i] + (long long)step * 2048 + h * 1024, to + (wave * WL + i) * 2048 + h * 1024);
-#pragma unroll
-    for (int i = 0; i < XL; ++i)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int at = step * 128 + h * 64;
-        if (ALIGNED) load_to_lds(at + g * 16 < a.kbytes ? xsrc[i] + at : a.zeros, to + (BN + wave * XL + i) * 2048 + h * 1024);
-        else xr[i][h] = load_part<P::elem>(xsrc[i] + at, a.kbytes - at - g * 16);
-      }
+      for (int i = 0; i < 2 * XL; ++i) xr[i] = load_part<P::elem>(xsrc[i] + step * 128, a.kbytes - step * 128 - part * 16);
+    }
   };
   auto put = [&](int stage) {
-    if (!ALIGNED) {
+    if constexpr (!ALIGNED) {
 #pragma unroll
-      for (int i = 0; i < XL; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<i4 *>(lds + stage * STAGE + (BN + wave * XL + i) * 2048 + h * 1024 + lane * 16) = xr[i][h];
+      for (int i = 0; i < 2 * XL; ++i) *reinterpret_cast<i4 *>(lds + stage * STAGE + (BN + wave * XL) * 2048 + i * 1024 + lane * 16) = xr[i];
     }
   };
 
-  const int wn = wave % WN, wm = wave / WN;
   Acc acc[NTW][MTW];
 #pragma unroll
   for (int n = 0; n < NTW; ++n)
 #pragma unroll
     for (int m = 0; m < MTW; ++m) acc[n][m] = Acc{0, 0, 0, 0};
+  i4 wq[2][NTW], xq[2][MTW];   // the operands of the two halves
 
-  load(0, 0);
-  put(0);
-  for (int step = 0; step < steps; ++step) {
-    const int stage = step & 1;
+  auto read = [&](int j, int stage, int h) {   // the j-th of a half's operands
+    if (j < MTW) xq[h][j < MTW ? j : 0] = *reinterpret_cast<const i4 *>(xlds + stage * STAGE + j * 2048 + (xpart ^ (h * 64)));
+    else if (j < MTW + NTW) wq[h][j - MTW < NTW ? j - MTW : 0] = *reinterpret_cast<const i4 *>(wlds + stage * STAGE + (j - MTW) * 2048 + h * 1024);
+  };
+  // the products of half h, between them the reads of the other half (of step `from`) and, behind the meeting, loads
+  auto half = [&](int h, int from, int step, bool loads) {
+    constexpr int PER = (LOADS + NTW - 1) / NTW;
+#pragma unroll
+    for (int n = 0; n < NTW; ++n) {
+      if (loads) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j)
+          if (n * PER + j < LOADS) load(n * PER + j, step, step & 1);
+      }
+      read(2 * n, from & 1, h ^ 1);
+      read(2 * n + 1, from & 1, h ^ 1);
+#pragma unroll
+      for (int m = 0; m < MTW; ++m) acc[n][m] = P::mma(wq[h][n], xq[h][m], acc[n][m]);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+  auto meet = [&]() {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
     __builtin_amdgcn_s_barrier();
-    if (step + 1 < steps) load(step + 1, stage ^ 1);
-    const char *wl = lds + stage * STAGE + wn * NTW * 2048 + lane * 16;
-    const char *xl = lds + stage * STAGE + (BN + wm * MTW) * 2048 + lane * 16;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i4 wq[NTW], xq[MTW];
-#pragma unroll
-      for (int m = 0; m < MTW; ++m) xq[m] = *reinterpret_cast<const i4 *>(xl + m * 2048 + h * 1024);
-#pragma unroll
-      for (int n = 0; n < NTW; ++n) wq[n] = *reinterpret_cast<const i4 *>(wl + n * 2048 + h * 1024);
-#pragma unroll
-      for (int n = 0; n < NTW; ++n)
-#pragma unroll
-        for (int m = 0; m < MTW; ++m) acc[n][m] = P::mma(wq[n], xq[m], acc[n][m]);
-    }
-    if (step + 1 < steps) put(stage ^ 1);
-  }
+    asm volatile("" : : : "memory");
+  };
 
 #pragma unroll
-  for (int m = 0; m < MTW; ++m) {
-    const long long p = blk.first + (wm * MTW + m) * 16 + c;
-    if (p >= blk.last) continue;
-    const RowOf row = row_of(a, p);
-    if (!row.there) continue;
-    const float xs = a.xscale ? a.xscale[row.in] : 1.0f;
-    char *orow = a.out + row.out * a.ldo;
-    const char *rrow = a.res ? a.res + row.out * a.ldr : nullptr;
+  for (int j = 0; j < LOADS; ++j) load(j, 0, 0);
+  fetch(0);
+  put(0);
+  if (steps > 1) {
 #pragma unroll
-    for (int n = 0; n < NTW; n += 4) {
-      const int tile = bn * BN + wn * NTW + n;
-      if (tile >= a.tiles) continue;
-      const long long at = ((long long)blk.expert * a.tiles + tile) * 16 + g * 4;
-      if (a.gated) {
-        float v[8];
+    for (int j = 0; j < LOADS; ++j) load(j, 1, 1);
+    fetch(1);
+    put(1);
+  }
+  meet();
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const f4 gate = finish_sums(a, acc[n + 2 * u][m], at + 32 * u, xs), up = finish_sums(a, acc[n + 2 * u + 1][m], at + 32 * u + 16, xs);
+  for (int j = 0; j < MTW + NTW; ++j) read(j, 0, 0);
+  int step = 0;
+  for (; step + 2 < steps; ++step) {
+    fetch(step + 2);
+    half(0, step, 0, false);
+    meet();
+    put(step & 1);
+    half(1, step + 1, step + 2, true);
+  }
+  for (; step < steps; ++step) {
+    half(0, step, 0, false);
+    meet();
+    half(1, step + 1, 0, false);
+  }
+
+  // The results go through LDS, 16 rows of every wave at a time, and come back as runs of 8 columns a thread: a wave then has
+  // whole rows of results beside each other in memory, and one short piece of code has every form of the epilogue.
+  constexpr int ROW = BN * 64 + 16, THREADS = WAVES * 64;   // bytes of a row: its last 16 keep rows off each other's banks
+  static_assert(WM * 16 * ROW <= 2 * STAGE, "16 rows of every wave fit");
+  const int units = a.gated ? BN : 2 * BN;   // runs of 8 results in a row
+  const int unit = threadIdx.x % units, row0 = threadIdx.x / units;
+  // packed rows of the run: those of its first 4 columns and of the next 4 (gated: of the gates; the partners are 16 behind)
+  const int tile = bn * BN + (a.gated ? unit / 4 : unit / 8) * 4;
+  const int col = a.gated ? (tile >> 2) * 32 + unit % 4 * 8 : (tile >> 2) * 64 + unit % 8 * 8;
+  const int at0 = a.gated ? unit % 4 * 4 : unit % 2 * 32 + unit % 8 / 2 * 4, step1 = a.gated ? 32 : 16, pair = a.gated ? 16 : 0;
+  const bool live = tile < a.tiles && col < a.oc;
+  const long long at = ((long long)blk.expert * a.tiles + (live ? tile : 0)) * 16 + at0;
+  // (a run's columns are 32 bytes of f32 in LDS; gated: the 32 gates of a group of 64 come before their partners)
+  const int from = a.gated ? unit / 4 * 256 + unit % 4 * 32 : unit * 32;
+  f4 ws[2][2], bias[2][2];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[4 * u + r] = activate(gate[r], a.act) * up[r];
-        }
-        store_columns<8>(a, v, orow, rrow, (tile >> 2) * 32 + g * 8);
-      } else {
-        float v[16];
+  for (int q = 0; q < 2; ++q)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const f4 s = finish_sums(a, acc[n + t][m], at + 16 * t, xs);
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[4 * t + r] = activate(s[r], a.act);
-        }
-        store_columns<16>(a, v, orow, rrow, (tile >> 2) * 64 + g * 16);
-      }
+    for (int t = 0; t < 2; ++t) {
+      if (a.wscale) ws[q][t] = *reinterpret_cast<const f4 *>(a.wscale + at + q * step1 + t * pair);
+      if (a.bias) bias[q][t] = *reinterpret_cast<const f4 *>(a.bias + at + q * step1 + t * pair);
     }
+  __syncthreads();
+#pragma unroll 1
+  for (int m = 0; m < MTW; ++m) {
+    char *to = lds + (wm * 16 + c) * ROW;
+#pragma unroll
+    for (int n = 0; n < NTW; ++n) {
+      const int t = wn * NTW + n, in_group = a.gated ? t % 2 * 128 + g * 32 + t % 4 / 2 * 16 : g * 64 + t % 4 * 16;
+      Acc v = acc[n][0];
+#pragma unroll
+      for (int k = 1; k < MTW; ++k) v = m == k ? acc[n][k] : v;
+      *reinterpret_cast<Acc *>(to + t / 4 * 256 + in_group) = v;
+    }
+    __syncthreads();
+    for (int r = row0; r < WM * 16; r += THREADS / units) {
+      const long long p = blk.first + (r / 16 * MTW + m) * 16 + r % 16;
+      if (!live || p >= blk.last) continue;
+      const RowOf row = row_of(a, p);
+      if (!row.there) continue;
+      const float xs = a.xscale ? a.xscale[row.in] : 1.0f;
+      float v[2][8];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (t && !a.gated) break;
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          const Acc s = *reinterpret_cast<const Acc *>(lds + r * ROW + from + t * 128 + q * 16);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float f = (float)s[j];
+            if (a.wscale) f *= xs * ws[q][t][j];
+            if (a.bias) f += bias[q][t][j];
+            v[t][4 * q + j] = f;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[0][j] = activate(v[0][j], a.act);
+      if (a.gated) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[0][j] *= v[1][j];
+      }
+      store_columns<8>(a, v[0], a.out + row.out * a.ldo, a.res ? a.res + row.out * a.ldr : nullptr, col);
+    }
+    __syncthreads();
   }
 }
 
