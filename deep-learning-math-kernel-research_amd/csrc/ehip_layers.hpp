@@ -151,13 +151,47 @@ template <> struct Product<EHIP_S8> {
   __device__ static __forceinline__ Acc mma(i4 w, i4 x, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0); }
 };
 
-__device__ __forceinline__ float activate(float v, int act)
+// The activation functions in single precision.
+// GELU: v * Phi(v), Phi by the complementary error function e of |v| / sqrt(2): a polynomial of degree 5 in 1 / (1 + p z) times
+// exp(-z^2) (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26, off by at most 1.5e-7), so |v| / 2 times that: two
+// transcendental instructions in the place of a library call of dozens.
+// SiLU: the exponential of a large negative v is infinite and the result -0, as the limit is.
+template <int ACT>
+__device__ __forceinline__ float activate(float v)
 {
-  if (act == EHIP_ACT_RELU) return v > 0.0f ? v : v != v ? v : 0.0f;
-  if (act == EHIP_ACT_GELU) return 0.5f * v * (1.0f + erff(v * 0.70710678118654752f));
-  // the exponential of a large negative v is infinite and the quotient -0, as the limit is
-  if (act == EHIP_ACT_SILU) return v / (1.0f + __expf(-v));
+  if (ACT == EHIP_ACT_RELU) return v > 0.0f ? v : v != v ? v : 0.0f;
+  if (ACT == EHIP_ACT_GELU) {
+    const float z = __builtin_fabsf(v) * 0.70710678118654752f, t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, z, 1.0f));
+    float e = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
+    e = __builtin_fmaf(t, e, 1.421413741f);
+    e = __builtin_fmaf(t, e, -0.284496736f);
+    e = __builtin_fmaf(t, e, 0.254829592f) * t * __builtin_amdgcn_exp2f(-1.4426950408889634f * z * z);
+    const float half = 0.5f * (v > 20.0f ? 20.0f : v) * e;   // (e is 0 by then: v = inf stays clear of inf * 0)
+    return v >= 0.0f ? v - half : half;
+  }
+  if (ACT == EHIP_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));
   return v;
+}
+// f(integral constants of the activation, the output type and whether it is gated): code for each, chosen once
+template <int V> struct Const {
+  static constexpr int value = V;
+};
+template <typename F>
+__device__ __forceinline__ void for_epilogue(const LinearArgs &a, F f)
+{
+  auto with_act = [&](auto act) {
+    auto with_type = [&](auto type) {
+      if (a.gated) f(act, type, Const<1>());
+      else f(act, type, Const<0>());
+    };
+    if (a.out_type == EHIP_BF16) with_type(Const<EHIP_BF16>());
+    else if (a.out_type == EHIP_F16) with_type(Const<EHIP_F16>());
+    else with_type(Const<EHIP_F32>());
+  };
+  if (a.act == EHIP_ACT_NONE) with_act(Const<EHIP_ACT_NONE>());
+  else if (a.act == EHIP_ACT_SILU) with_act(Const<EHIP_ACT_SILU>());
+  else if (a.act == EHIP_ACT_GELU) with_act(Const<EHIP_ACT_GELU>());
+  else with_act(Const<EHIP_ACT_RELU>());
 }
 
 // a tile's sums of one lane as f32: scaled (s8), with bias.  at: the lane's first row in the packed order
@@ -178,23 +212,19 @@ __device__ __forceinline__ f4 finish_sums(const LinearArgs &a, Acc acc, long lon
   return v;
 }
 
-// N (a multiple of 4) columns beside each other of one row, from column `col` on: residual, rounding, store.  Columns past the
-// last are dropped.
-template <int N>
-__device__ __forceinline__ void store_columns(const LinearArgs &a, float (&v)[N], char *orow, const char *rrow, int col)
+// N (a multiple of 4) columns beside each other of one row at o (its residual at r, or null): residual, rounding, store.  Only
+// the first n exist.
+template <int TYPE, int N>
+__device__ __forceinline__ void store_columns(float (&v)[N], char *o, const char *r, float res_scale, int n)
 {
-  const int size = a.out_type == EHIP_F32 ? 4 : 2;
-  const bool bf16 = a.out_type == EHIP_BF16;
-  char *o = orow + (long long)col * size;
-  const char *r = rrow ? rrow + (long long)col * size : nullptr;
-  const int n = a.oc - col;
+  constexpr int SIZE = TYPE == EHIP_F32 ? 4 : 2;
   if (n < N) {
 #pragma unroll
     for (int q = 0; q < N; ++q)
-      if (q < n) store_one(o + q * size, a.out_type, r ? __builtin_fmaf(a.res_scale, load_one(r + q * size, a.out_type), v[q]) : v[q]);
+      if (q < n) store_one(o + q * SIZE, TYPE, r ? __builtin_fmaf(res_scale, load_one(r + q * SIZE, TYPE), v[q]) : v[q]);
     return;
   }
-  if (a.out_type == EHIP_F32) {
+  if constexpr (TYPE == EHIP_F32) {
     typedef float fu __attribute__((ext_vector_type(4), aligned(4)));
 #pragma unroll
     for (int q = 0; q < N; q += 4) {
@@ -202,31 +232,32 @@ __device__ __forceinline__ void store_columns(const LinearArgs &a, float (&v)[N]
       if (r) {
         const fu old = *reinterpret_cast<const fu *>(r + 4 * q);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) s[j] = __builtin_fmaf(a.res_scale, old[j], s[j]);
+        for (int j = 0; j < 4; ++j) s[j] = __builtin_fmaf(res_scale, old[j], s[j]);
       }
       *reinterpret_cast<fu *>(o + 4 * q) = s;
     }
-    return;
-  }
-  // 4 columns of 16 bits are 8 bytes, 8 are 16
-  constexpr int STEP = N % 8 == 0 ? 8 : 4;
-  typedef unsigned dw __attribute__((ext_vector_type(STEP / 2), aligned(2)));
+  } else {
+    // 4 columns of 16 bits are 8 bytes, 8 are 16
+    constexpr int STEP = N % 8 == 0 ? 8 : 4;
+    typedef unsigned dw __attribute__((ext_vector_type(STEP / 2), aligned(2)));
 #pragma unroll
-  for (int q = 0; q < N; q += STEP) {
-    if (r) {
-      const dw old = *reinterpret_cast<const dw *>(r + 2 * q);
+    for (int q = 0; q < N; q += STEP) {
+      if (r) {
+        const dw old = *reinterpret_cast<const dw *>(r + 2 * q);
 #pragma unroll
-      for (int j = 0; j < STEP / 2; ++j) {
-        float lo, hi;
-        unpack(old[j], bf16, lo, hi);
-        v[q + 2 * j] = __builtin_fmaf(a.res_scale, lo, v[q + 2 * j]);
-        v[q + 2 * j + 1] = __builtin_fmaf(a.res_scale, hi, v[q + 2 * j + 1]);
+        for (int j = 0; j < STEP / 2; ++j) {
+          float lo, hi;
+          unpack(old[j], TYPE == EHIP_BF16, lo, hi);
+          v[q + 2 * j] = __builtin_fmaf(res_scale, lo, v[q + 2 * j]);
+          v[q + 2 * j + 1] = __builtin_fmaf(res_scale, hi, v[q + 2 * j + 1]);
+        }
       }
-    }
-    dw p;
+      dw p;
 #pragma unroll
-    for (int j = 0; j < STEP / 2; ++j) p[j] = bf16 ? pack_bf16(v[q + 2 * j], v[q + 2 * j + 1]) : pack_f16(v[q + 2 * j], v[q + 2 * j + 1]);
-    *reinterpret_cast<dw *>(o + 2 * q) = p;
+      for (int j = 0; j < STEP / 2; ++j)
+        p[j] = TYPE == EHIP_BF16 ? pack_bf16(v[q + 2 * j], v[q + 2 * j + 1]) : pack_f16(v[q + 2 * j], v[q + 2 * j + 1]);
+      *reinterpret_cast<dw *>(o + 2 * q) = p;
+    }
   }
 }
 

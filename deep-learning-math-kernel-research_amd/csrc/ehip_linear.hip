@@ -154,33 +154,36 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_split(LinearArgs a)
     return s;
   };
   constexpr int PAIRS = NT > 1 ? NT / 2 : 1;
-  const int units = (a.gated ? PAIRS : NT) * MT;
-  for (int i = wave; i < units; i += WAVES) {
-    const int m = i % MT, n = i / MT;
-    const long long p = blk.first + m * 16 + c;
-    if (p >= blk.last) continue;
-    const RowOf row = row_of(a, p);
-    if (!row.there) continue;
-    const float xs = a.xscale ? a.xscale[row.in] : 1.0f;
-    float v[4];
-    int col;
-    if (a.gated) {
-      const int tile = tile0 + 2 * n;
-      const long long at = ((long long)blk.expert * a.tiles + tile) * 16 + g * 4;
-      const f4 gate = finish_sums(a, total(2 * n, m), at, xs);
-      const f4 up = finish_sums(a, total(NT > 1 ? 2 * n + 1 : 0, m), at + 16, xs);
+  for_epilogue(a, [&](auto act, auto type, auto gated) {
+    constexpr int UNITS = (gated.value ? PAIRS : NT) * MT, SIZE = type.value == EHIP_F32 ? 4 : 2;
+    for (int i = wave; i < UNITS; i += WAVES) {
+      const int m = i % MT, n = i / MT;
+      const long long p = blk.first + m * 16 + c;
+      if (p >= blk.last) continue;
+      const RowOf row = row_of(a, p);
+      if (!row.there) continue;
+      const float xs = a.xscale ? a.xscale[row.in] : 1.0f;
+      float v[4];
+      int col;
+      if constexpr (gated.value) {
+        const int tile = tile0 + 2 * n;
+        const long long at = ((long long)blk.expert * a.tiles + tile) * 16 + g * 4;
+        const f4 gate = finish_sums(a, total(2 * n, m), at, xs);
+        const f4 up = finish_sums(a, total(NT > 1 ? 2 * n + 1 : 0, m), at + 16, xs);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = activate(gate[r], a.act) * up[r];
-      col = (tile >> 2) * 32 + g * 8 + ((tile & 3) >> 1) * 4;
-    } else {
-      const int tile = tile0 + n;
-      const f4 t = finish_sums(a, total(n, m), ((long long)blk.expert * a.tiles + tile) * 16 + g * 4, xs);
+        for (int r = 0; r < 4; ++r) v[r] = activate<act.value>(gate[r]) * up[r];
+        col = (tile >> 2) * 32 + g * 8 + ((tile & 3) >> 1) * 4;
+      } else {
+        const int tile = tile0 + n;
+        const f4 t = finish_sums(a, total(n, m), ((long long)blk.expert * a.tiles + tile) * 16 + g * 4, xs);
 #pragma unroll
-      for (int r = 0; r < 4; ++r) v[r] = activate(t[r], a.act);
-      col = (tile >> 2) * 64 + g * 16 + (tile & 3) * 4;
+        for (int r = 0; r < 4; ++r) v[r] = activate<act.value>(t[r]);
+        col = (tile >> 2) * 64 + g * 16 + (tile & 3) * 4;
+      }
+      store_columns<type.value, 4>(v, a.out + row.out * a.ldo + (long long)col * SIZE,
+                                   a.res ? a.res + row.out * a.ldr + (long long)col * SIZE : nullptr, a.res_scale, a.oc - col);
     }
-    store_columns<4>(a, v, a.out + row.out * a.ldo, a.res ? a.res + row.out * a.ldr : nullptr, col);
-  }
+  });
 }
 
 namespace {

@@ -149,72 +149,78 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
   }
 
   // The results go through LDS, 16 rows of every wave at a time, and come back as runs of 8 columns a thread: a wave then has
-  // whole rows of results beside each other in memory, and one short piece of code has every form of the epilogue.
+  // whole rows of results beside each other in memory.
   constexpr int ROW = BN * 64 + 16, THREADS = WAVES * 64;   // bytes of a row: its last 16 keep rows off each other's banks
   static_assert(WM * 16 * ROW <= 2 * STAGE, "16 rows of every wave fit");
-  const int units = a.gated ? BN : 2 * BN;   // runs of 8 results in a row
-  const int unit = threadIdx.x % units, row0 = threadIdx.x / units;
-  // packed rows of the run: those of its first 4 columns and of the next 4 (gated: of the gates; the partners are 16 behind)
-  const int tile = bn * BN + (a.gated ? unit / 4 : unit / 8) * 4;
-  const int col = a.gated ? (tile >> 2) * 32 + unit % 4 * 8 : (tile >> 2) * 64 + unit % 8 * 8;
-  const int at0 = a.gated ? unit % 4 * 4 : unit % 2 * 32 + unit % 8 / 2 * 4, step1 = a.gated ? 32 : 16, pair = a.gated ? 16 : 0;
-  const bool live = tile < a.tiles && col < a.oc;
-  const long long at = ((long long)blk.expert * a.tiles + (live ? tile : 0)) * 16 + at0;
-  // (a run's columns are 32 bytes of f32 in LDS; gated: the 32 gates of a group of 64 come before their partners)
-  const int from = a.gated ? unit / 4 * 256 + unit % 4 * 32 : unit * 32;
-  f4 ws[2][2], bias[2][2];
+  for_epilogue(a, [&](auto act, auto type, auto gated) {
+    constexpr bool GATED = gated.value;
+    constexpr int SIZE = type.value == EHIP_F32 ? 4 : 2;
+    constexpr int UNITS = GATED ? BN : 2 * BN, HIGH = THREADS / UNITS;   // runs of 8 results in a row; rows at a time
+    static_assert(HIGH % 16 == 0 && WM * 16 % HIGH == 0, "a thread's rows are a multiple of 16 apart");
+    const int unit = threadIdx.x % UNITS, row0 = threadIdx.x / UNITS;
+    // packed rows of the run: those of its first 4 columns and of the next 4 (gated: of the gates; the partners are 16 behind)
+    const int tile = bn * BN + (GATED ? unit / 4 : unit / 8) * 4;
+    const int col = GATED ? (tile >> 2) * 32 + unit % 4 * 8 : (tile >> 2) * 64 + unit % 8 * 8;
+    const bool live = tile < a.tiles && col < a.oc;
+    const long long at = ((long long)blk.expert * a.tiles + (live ? tile : 0)) * 16 + (GATED ? unit % 4 * 4 : unit % 2 * 32 + unit % 8 / 2 * 4);
+    f4 ws[2][1 + GATED], bias[2][1 + GATED];
 #pragma unroll
-  for (int q = 0; q < 2; ++q)
+    for (int q = 0; q < 2; ++q)
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (a.wscale) ws[q][t] = *reinterpret_cast<const f4 *>(a.wscale + at + q * step1 + t * pair);
-      if (a.bias) bias[q][t] = *reinterpret_cast<const f4 *>(a.bias + at + q * step1 + t * pair);
-    }
-  __syncthreads();
-#pragma unroll 1
-  for (int m = 0; m < MTW; ++m) {
-    char *to = lds + (wm * 16 + c) * ROW;
+      for (int t = 0; t <= GATED; ++t) {
+        if (a.wscale) ws[q][t] = *reinterpret_cast<const f4 *>(a.wscale + at + q * (GATED ? 32 : 16) + t * 16);
+        if (a.bias) bias[q][t] = *reinterpret_cast<const f4 *>(a.bias + at + q * (GATED ? 32 : 16) + t * 16);
+      }
+    // (a run's columns are 32 bytes of f32 in LDS; gated: the 32 gates of a group of 64 come before their partners)
+    const char *from = lds + row0 * ROW + (GATED ? unit / 4 * 256 + unit % 4 * 32 : unit * 32);
+    char *to = lds + (wm * 16 + c) * ROW + (GATED ? g * 32 : g * 64);
+    auto write = [&](auto mc) {
 #pragma unroll
-    for (int n = 0; n < NTW; ++n) {
-      const int t = wn * NTW + n, in_group = a.gated ? t % 2 * 128 + g * 32 + t % 4 / 2 * 16 : g * 64 + t % 4 * 16;
-      Acc v = acc[n][0];
+      for (int n = 0; n < NTW; ++n) {
+        const int t = wn * NTW + n;
+        *reinterpret_cast<Acc *>(to + t / 4 * 256 + (GATED ? t % 2 * 128 + t % 4 / 2 * 16 : t % 4 * 16)) = acc[n][mc.value];
+      }
+    };
+    auto read = [&](int m) {
 #pragma unroll
-      for (int k = 1; k < MTW; ++k) v = m == k ? acc[n][k] : v;
-      *reinterpret_cast<Acc *>(to + t / 4 * 256 + in_group) = v;
-    }
-    __syncthreads();
-    for (int r = row0; r < WM * 16; r += THREADS / units) {
-      const long long p = blk.first + (r / 16 * MTW + m) * 16 + r % 16;
-      if (!live || p >= blk.last) continue;
-      const RowOf row = row_of(a, p);
-      if (!row.there) continue;
-      const float xs = a.xscale ? a.xscale[row.in] : 1.0f;
-      float v[2][8];
+      for (int k = 0; k < WM * 16 / HIGH; ++k) {
+        const long long p = blk.first + ((row0 / 16 + k * (HIGH / 16)) * MTW + m) * 16 + row0 % 16;
+        const RowOf row = p < blk.last ? row_of(a, p) : RowOf{0, 0, false};
+        if (!live || !row.there) continue;
+        const float xs = a.xscale ? a.xscale[row.in] : 1.0f;
+        float v[1 + GATED][8];
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (t && !a.gated) break;
+        for (int t = 0; t <= GATED; ++t)
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
-          const Acc s = *reinterpret_cast<const Acc *>(lds + r * ROW + from + t * 128 + q * 16);
+          for (int q = 0; q < 2; ++q) {
+            const Acc s = *reinterpret_cast<const Acc *>(from + k * HIGH * ROW + t * 128 + q * 16);
+            f4 f = {(float)s[0], (float)s[1], (float)s[2], (float)s[3]};
+            if (a.wscale) f *= xs * ws[q][t];
+            if (a.bias) f += bias[q][t];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            float f = (float)s[j];
-            if (a.wscale) f *= xs * ws[q][t][j];
-            if (a.bias) f += bias[q][t][j];
-            v[t][4 * q + j] = f;
+            for (int j = 0; j < 4; ++j) v[t][4 * q + j] = f[j];
           }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          v[0][j] = activate<act.value>(v[0][j]);
+          if (GATED) v[0][j] *= v[GATED][j];
         }
+        store_columns<type.value, 8>(v[0], a.out + row.out * a.ldo + (long long)col * SIZE,
+                                     a.res ? a.res + row.out * a.ldr + (long long)col * SIZE : nullptr, a.res_scale, a.oc - col);
       }
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[0][j] = activate(v[0][j], a.act);
-      if (a.gated) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[0][j] *= v[1][j];
-      }
-      store_columns<8>(a, v[0], a.out + row.out * a.ldo, a.res ? a.res + row.out * a.ldr : nullptr, col);
-    }
-    __syncthreads();
-  }
+    };
+    auto pass = [&](auto mc) {
+      __syncthreads();
+      write(mc);
+      __syncthreads();
+      read(mc.value);
+    };
+    static_assert(MTW == 4, "four passes");
+    pass(Const<0>());
+    pass(Const<1>());
+    pass(Const<2>());
+    pass(Const<3>());
+  });
 }
 
 namespace {
