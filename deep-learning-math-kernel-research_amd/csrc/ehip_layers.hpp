@@ -62,7 +62,8 @@ hipError_t launch_norm(const NormArgs &a, int type, int out_s8, hipStream_t s);
 struct RouteArgs {
   int32_t *ids;
   float *weights;
-  int32_t *offsets, *slots, *hist;   // hist: [blocks of kRouteBlock tokens][experts]
+  int32_t *offsets, *slots;
+  int32_t *totals, *hist;   // [experts]; [experts][blocks of kRouteBlock tokens]
   const char *logits;
   const float *bias;
   long long tokens, ld;   // ld in bytes

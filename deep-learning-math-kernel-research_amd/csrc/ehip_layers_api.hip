@@ -341,7 +341,8 @@ EHIP_API int ehip_route_destroy(ehip_route_t *h)
 EHIP_API int64_t ehip_route_plan_ints(const ehip_route_t *h, int64_t tokens)
 {
   if (!h || tokens < 0 || tokens * h->d.topk >= 1ll << 30 || tokens >= 1ll << 30) return -1;
-  return h->d.experts + 1 + tokens * h->d.topk + (tokens + kRouteBlock - 1) / kRouteBlock * h->d.experts;
+  const int64_t kept = tokens > kRouteBlock ? (1 + (tokens + kRouteBlock - 1) / kRouteBlock) * h->d.experts : 0;
+  return h->d.experts + 1 + tokens * h->d.topk + kept;
 }
 
 EHIP_API int ehip_route_execute(const ehip_route_t *h, const ehip_route_args_t *args, void *hip_stream)
@@ -363,7 +364,8 @@ EHIP_API int ehip_route_execute(const ehip_route_t *h, const ehip_route_args_t *
     if (g.plan_dev) {
       a.offsets = g.plan_dev;
       a.slots = a.offsets + d.experts + 1;
-      a.hist = a.slots + g.tokens * d.topk;
+      a.totals = a.slots + g.tokens * d.topk;
+      a.hist = a.totals + d.experts;
     }
     a.logits = static_cast<const char *>(g.logits_dev);
     a.bias = g.bias_dev;

@@ -1,9 +1,12 @@
 // The experts of each token, and the order of their work.
 //
 // A wave has a token, its lanes the experts in runs of PER.  Every score is the definition's single-precision value: exp, the
-// sum over the experts in 64 bits (so that its order cannot show), one division; a choice is the largest key, by a maximum over
-// the wave, of the lowest expert that has it.  The slots of an expert keep the order of the tokens: workgroups count theirs,
-// and a second kernel places each behind those of the workgroups before it.  A few tokens take one workgroup and one launch.
+// sum over the experts in 64 bits (so that its order cannot show), one division.  A lane sorts its keys once; a choice is the
+// largest of the lanes' first ones, by the lowest lane that has it, which goes on to its next.  Reductions over the lanes are
+// cross-lane operands of vector instructions: through LDS each of their steps would cost its latency, 99 us where this takes
+// 21 (32768 tokens, 256 experts in 8 groups, 8 choices).
+// The slots of an expert keep the order of the tokens: workgroups count theirs, a kernel sums the counts over the workgroups
+// before each, a third places the slots.  A few tokens take one workgroup and one launch.
 #include "ehip_layers.hpp"
 
 namespace ehip {
@@ -11,137 +14,253 @@ namespace {
 
 constexpr float kClosed = -__builtin_inff();
 
-__device__ __forceinline__ float max_over_wave(float v)
+// v of the lane that DPP control CTRL names; lanes without one, or outside of ROWS, keep `old`
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int dpp(int old, int v)
 {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = fmaxf(v, __shfl_xor(v, d));
-  return v;
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float old, float v)
+{
+  return __builtin_bit_cast(float, dpp<CTRL, ROWS>(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v)));
+}
+constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143;
+
+// Keys are compared as integers of the same order (a zero has no sign): one instruction each, where a maximum of floats takes
+// three to keep a signalling NaN quiet.
+__device__ __forceinline__ int ordered(float v)
+{
+  const int b = __builtin_bit_cast(int, v + 0.0f);
+  return b ^ ((b >> 31) & 0x7fffffff);
+}
+__device__ __forceinline__ float unordered(int k) { return __builtin_bit_cast(float, k ^ ((k >> 31) & 0x7fffffff)); }
+constexpr int kClosedKey = (int)0x807fffff;   // ordered(-inf)
+__device__ __forceinline__ int imax(int a, int b) { return a > b ? a : b; }
+__device__ __forceinline__ int imin(int a, int b) { return a < b ? a : b; }
+
+// the maximum over the wave, in every lane (a scalar)
+__device__ __forceinline__ int max_over_wave(int v)
+{
+  v = imax(v, dpp<kShr1>(v, v));
+  v = imax(v, dpp<kShr2>(v, v));
+  v = imax(v, dpp<kShr4>(v, v));
+  v = imax(v, dpp<kShr8>(v, v));
+  v = imax(v, dpp<kBcast15, 0xa>(v, v));
+  v = imax(v, dpp<kBcast31, 0xc>(v, v));
+  return __builtin_amdgcn_readlane(v, 63);
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ double plus(double v)
+{
+  const long long b = __builtin_bit_cast(long long, v);
+  const int lo = dpp<CTRL, ROWS>(0, (int)b), hi = dpp<CTRL, ROWS>(0, (int)(b >> 32));
+  return v + __builtin_bit_cast(double, (long long)(unsigned)lo | ((long long)hi << 32));
+}
+__device__ __forceinline__ double sum_over_wave(double v)
+{
+  v = plus<kShr1>(v);
+  v = plus<kShr2>(v);
+  v = plus<kShr4>(v);
+  v = plus<kShr8>(v);
+  v = plus<kBcast15, 0xa>(v);
+  v = plus<kBcast31, 0xc>(v);
+  const long long b = __builtin_bit_cast(long long, v);
+  const int lo = __builtin_amdgcn_readlane((int)b, 63), hi = __builtin_amdgcn_readlane((int)(b >> 32), 63);
+  return __builtin_bit_cast(double, (long long)(unsigned)lo | ((long long)hi << 32));
 }
 
-// One token: lane j < topk returns its j-th choice (-1: none) and that choice's weight
 template <int TYPE, int PER>
-__device__ __forceinline__ void choose(const RouteArgs &a, long long token, float *keys, int *id_out, float *weight_out)
+__device__ __forceinline__ void load_logits(const RouteArgs &a, long long token, float (&x)[PER])
 {
-  const int lane = threadIdx.x & 63, first = lane * PER;
   constexpr int size = TYPE == EHIP_F32 ? 4 : 2;
+  const int first = (threadIdx.x & 63) * PER;
   const char *row = a.logits + token * a.ld + (long long)first * size;
-  float x[PER], score[PER], key[PER];
-  float top = kClosed;
+  if (first + PER <= a.experts) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = load_one(row + j * size, TYPE);
+    return;
+  }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) x[j] = first + j < a.experts ? load_one(row + j * size, TYPE) : kClosed;
+}
+
+// How the groups lie over a wave: 64 / (groups rounded up to a power of two) lanes look through one
+template <int PER> struct Groups {
+  int size, lanes, mine;
+  bool own;             // each lane's keys are of the group that it looks through
+  unsigned char at[PER];   // lane that speaks for the group of each of the lane's experts
+};
+template <int PER>
+__device__ __forceinline__ Groups<PER> groups_of(const RouteArgs &a)
+{
+  Groups<PER> g;
+  const int lane = threadIdx.x & 63;
+  g.size = a.experts / a.groups;
+  g.lanes = 64;
+  while (g.lanes * a.groups > 64) g.lanes >>= 1;
+  g.mine = lane / g.lanes;
+  g.own = g.lanes * PER == g.size;
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    x[j] = kClosed;
-    if (first + j < a.experts) x[j] = load_one(row + j * size, TYPE);
-    if (!(x[j] > kClosed)) x[j] = kClosed;   // a NaN
-    x[j] = fminf(x[j], 3.402823466e38f);
-    top = fmaxf(top, x[j]);
+    const int e = lane * PER + j;
+    g.at[j] = (unsigned char)(e < a.experts ? e / g.size * g.lanes : 0);
+  }
+  return g;
+}
+
+// the two largest of two pairs
+__device__ __forceinline__ void join(int &b1, int &b2, int o1, int o2)
+{
+  b2 = imax(imin(b1, o1), imax(b2, o2));
+  b1 = imax(b1, o1);
+}
+
+// One token from its logits: lane j < topk returns its j-th choice (-1: none) and that choice's weight.  room: of the wave
+template <int PER>
+__device__ __forceinline__ void choose(const RouteArgs &a, const Groups<PER> &g, float (&x)[PER], float *room, int *id_out, float *weight_out)
+{
+  const int lane = threadIdx.x & 63, first = lane * PER;
+  float score[PER];
+  int key[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    x[j] = x[j] > kClosed ? x[j] : kClosed;   // a NaN is closed, too
+    x[j] = x[j] < 3.402823466e38f ? x[j] : 3.402823466e38f;
   }
   if (a.sigmoid) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) score[j] = 1.0f / (1.0f + expf(-x[j]));
   } else {
-    top = max_over_wave(top);
+    int most = ordered(x[0]);
+#pragma unroll
+    for (int j = 1; j < PER; ++j) most = imax(most, ordered(x[j]));
+    const float top = unordered(max_over_wave(most));
     double sum = 0.0;
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
       score[j] = x[j] > kClosed ? expf(x[j] - top) : 0.0f;
       sum += (double)score[j];
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-    const float all = (float)sum;
+    const float all = (float)sum_over_wave(sum);
 #pragma unroll
     for (int j = 0; j < PER; ++j) score[j] /= all;
   }
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    key[j] = kClosed;
-    if (x[j] > kClosed) {
-      key[j] = a.bias ? score[j] + a.bias[first + j] : score[j];
-      if (key[j] != key[j]) key[j] = kClosed;
-    }
+    float k = score[j];
+    if (a.bias && first + j < a.experts) k += a.bias[first + j];
+    key[j] = x[j] > kClosed && k == k ? ordered(k) : kClosedKey;
   }
 
   if (a.open < a.groups) {
-    // the best one or two keys of each group: 64 / (groups rounded up to a power of two) lanes look through one
-    const int size_g = a.experts / a.groups;
-    int lanes = 64;
-    while (lanes * a.groups > 64) lanes >>= 1;
+    // the best one or two keys of each group
+    int b1, b2 = kClosedKey;
+    if (g.own) {
+      b1 = key[0];
 #pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (first + j < a.experts) keys[first + j] = key[j];
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    const int mine = lane / lanes;
-    float b1 = kClosed, b2 = kClosed;
-    if (mine < a.groups)
-      for (int i = lane % lanes; i < size_g; i += lanes) {
-        const float k = keys[mine * size_g + i];
-        b2 = fmaxf(b2, fminf(b1, k));
-        b1 = fmaxf(b1, k);
-      }
-    for (int d = 1; d < lanes; d <<= 1) {
-      const float o1 = __shfl_xor(b1, d), o2 = __shfl_xor(b2, d);
-      b2 = fmaxf(fminf(b1, o1), fmaxf(b2, o2));
-      b1 = fmaxf(b1, o1);
+      for (int j = 1; j < PER; ++j) join(b1, b2, key[j], kClosedKey);
+    } else {
+#pragma unroll
+      for (int j = 0; j < PER; ++j) room[first + j] = __builtin_bit_cast(float, key[j]);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      b1 = kClosedKey;
+      if (g.mine < a.groups)
+        for (int i = lane % g.lanes; i < g.size; i += g.lanes) join(b1, b2, __builtin_bit_cast(int, room[g.mine * g.size + i]), kClosedKey);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (what is written into the room next comes after these reads)
     }
-    const float total = a.best > 1 && b2 > kClosed ? b1 + b2 : b1;
+    // lanes 1, 2, 4, 8 away: swaps in a quad, mirrors of 8 and 16 (whose halves agree in themselves by then)
+    if (g.lanes > 1) join(b1, b2, dpp<0xb1>(b1, b1), dpp<0xb1>(b2, b2));
+    if (g.lanes > 2) join(b1, b2, dpp<0x4e>(b1, b1), dpp<0x4e>(b2, b2));
+    if (g.lanes > 4) join(b1, b2, dpp<0x141>(b1, b1), dpp<0x141>(b2, b2));
+    if (g.lanes > 8) join(b1, b2, dpp<0x140>(b1, b1), dpp<0x140>(b2, b2));
+    if (g.lanes > 16) join(b1, b2, __shfl_xor(b1, 16), __shfl_xor(b2, 16));
+    if (g.lanes > 32) join(b1, b2, __shfl_xor(b1, 32), __shfl_xor(b2, 32));
+    const int total = a.best > 1 && b2 > kClosedKey ? ordered(unordered(b1) + unordered(b2)) : b1;
     int better = 0;
     for (int q = 0; q < a.groups; ++q) {
-      const float other = __shfl(total, q * lanes);
-      better += other > total || (other == total && q < mine);
+      const int other = __builtin_amdgcn_readlane(total, q * g.lanes);
+      better += other > total || (other == total && q < g.mine) ? 1 : 0;
     }
-    const unsigned long long open = __ballot(better < a.open && mine < a.groups);
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (the next token's keys come after these reads)
+    const unsigned long long open = __ballot(better < a.open && g.mine < a.groups);
 #pragma unroll
     for (int j = 0; j < PER; ++j)
-      if (first + j < a.experts && !((open >> ((first + j) / size_g * lanes)) & 1)) key[j] = kClosed;
+      if (!((open >> g.at[j]) & 1)) key[j] = kClosedKey;
   }
+#pragma unroll
+  for (int j = 0; j < PER; ++j) room[first + j] = score[j];
+
+  // exchanges of neighbours only, of unequal keys only: equal ones stay in the order of their experts
+  int expert[PER];
+#pragma unroll
+  for (int j = 0; j < PER; ++j) expert[j] = first + j;
+#pragma unroll
+  for (int i = 0; i < PER - 1; ++i)
+#pragma unroll
+    for (int j = PER - 2; j >= i; --j) {
+      const bool swap = key[j + 1] > key[j];
+      const int k = key[j];
+      const int e = expert[j];
+      key[j] = swap ? key[j + 1] : k;
+      expert[j] = swap ? expert[j + 1] : e;
+      key[j + 1] = swap ? k : key[j + 1];
+      expert[j + 1] = swap ? e : expert[j + 1];
+    }
 
   int id = -1;
-  float weight = 0.0f, total = 0.0f;
   for (int k = 0; k < a.topk; ++k) {
-    float best = key[0], its = score[0];
-    int at = 0;
+    const int m = max_over_wave(key[0]);
+    if (m == kClosedKey) break;
+    const int who = __builtin_ctzll(__ballot(key[0] == m));
+    const int e = __builtin_amdgcn_readlane(expert[0], who);
+    id = lane == k ? e : id;
+    const bool mine = lane == who;
 #pragma unroll
-    for (int j = 1; j < PER; ++j)
-      if (key[j] > best) {
-        best = key[j];
-        its = score[j];
-        at = j;
-      }
-    const float m = max_over_wave(best);
-    if (!(m > kClosed)) break;
-    const int who = __builtin_ctzll(__ballot(best == m));
-    const float w = __shfl(its, who);
-    const int e = who * PER + __shfl(at, who);
-    total += w;
-    if (lane == k) {
-      id = e;
-      weight = w;
+    for (int j = 0; j + 1 < PER; ++j) {
+      key[j] = mine ? key[j + 1] : key[j];
+      expert[j] = mine ? expert[j + 1] : expert[j];
     }
-#pragma unroll
-    for (int j = 0; j < PER; ++j)
-      if (lane == who && j == at) key[j] = kClosed;
+    key[PER - 1] = mine ? kClosedKey : key[PER - 1];
   }
-  if (a.renorm) weight = total > 0.0f ? weight / total : 0.0f;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  float weight = id >= 0 ? room[id] : 0.0f;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");   // (the next token's go there after this)
+  if (a.renorm) {
+    // up to 32 choices: the first two rows of 16 lanes
+    float total = weight;
+    total += dpp<kShr1>(0.0f, total);
+    total += dpp<kShr2>(0.0f, total);
+    total += dpp<kShr4>(0.0f, total);
+    total += dpp<kShr8>(0.0f, total);
+    const int bits = __builtin_bit_cast(int, total);
+    total = __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 15)) + __builtin_bit_cast(float, __builtin_amdgcn_readlane(bits, 31));
+    weight = total > 0.0f ? weight / total : 0.0f;
+  }
   *id_out = id;
   *weight_out = weight * a.scale;
 }
 
-// a workgroup has kRouteBlock tokens and counts the slots of each expert among them
+// a workgroup has kRouteBlock tokens and counts the slots of each expert among them: hist [experts][workgroups]
 template <int TYPE, int PER>
-__global__ __launch_bounds__(512) void k_route_choose(RouteArgs a)
+__global__ __launch_bounds__(1024) void k_route_choose(RouteArgs a)
 {
-  constexpr int WAVES = 8;
-  __shared__ float keys[WAVES][64 * PER];
+  constexpr int WAVES = 16;
+  __shared__ float room[WAVES][64 * PER];
   __shared__ int count[64 * PER];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (int e = threadIdx.x; e < a.experts; e += 512) count[e] = 0;
+  for (int e = threadIdx.x; e < a.experts; e += 64 * WAVES) count[e] = 0;
   __syncthreads();
   const long long from = (long long)blockIdx.x * kRouteBlock, to = from + kRouteBlock < a.tokens ? from + kRouteBlock : a.tokens;
+  const Groups<PER> groups = groups_of<PER>(a);
+  float x[PER], ahead[PER];
+  if (from + wave < to) load_logits<TYPE, PER>(a, from + wave, ahead);
   for (long long t = from + wave; t < to; t += WAVES) {
+#pragma unroll
+    for (int j = 0; j < PER; ++j) x[j] = ahead[j];
+    if (t + WAVES < to) load_logits<TYPE, PER>(a, t + WAVES, ahead);
     int id;
     float w;
-    choose<TYPE, PER>(a, t, keys[wave], &id, &w);
+    choose<PER>(a, groups, x, room[wave], &id, &w);
     if (lane < a.topk) {
       a.ids[t * a.topk + lane] = id;
       a.weights[t * a.topk + lane] = w;
@@ -150,7 +269,49 @@ __global__ __launch_bounds__(512) void k_route_choose(RouteArgs a)
   }
   if (!a.hist) return;
   __syncthreads();
-  for (int e = threadIdx.x; e < a.experts; e += 512) a.hist[(long long)blockIdx.x * a.experts + e] = count[e];
+  for (int e = threadIdx.x; e < a.experts; e += 64 * WAVES) a.hist[(long long)e * gridDim.x + blockIdx.x] = count[e];
+}
+
+// sum of v over the lanes before this one; *all: over the wave
+__device__ __forceinline__ int sum_before(int v, int *all)
+{
+  int s = v;
+  s += dpp<kShr1>(0, s);
+  s += dpp<kShr2>(0, s);
+  s += dpp<kShr4>(0, s);
+  s += dpp<kShr8>(0, s);
+  s += dpp<kBcast15, 0xa>(0, s);
+  s += dpp<kBcast31, 0xc>(0, s);
+  *all = __builtin_amdgcn_readlane(s, 63);
+  return s - v;
+}
+
+// one wave an expert: its counts over the workgroups before each, in place, and in totals[expert] all of them
+__global__ __launch_bounds__(256) void k_route_sum(RouteArgs a, int blocks)
+{
+  const int e = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+  if (e >= a.experts) return;
+  int32_t *hist = a.hist + (long long)e * blocks;
+  int before = 0;
+  for (int b0 = 0; b0 < blocks; b0 += 256) {   // four a lane
+    int n[4], own = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int b = b0 + lane * 4 + j;
+      n[j] = b < blocks ? hist[b] : 0;
+      own += n[j];
+    }
+    int all;
+    int at = before + sum_before(own, &all);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int b = b0 + lane * 4 + j;
+      if (b < blocks) hist[b] = at;
+      at += n[j];
+    }
+    before += all;
+  }
+  if (lane == 0) a.totals[e] = before;
 }
 
 // 64 slots beside each other in a wave: how many before a lane's have the same expert, and how many have it in all.
@@ -190,49 +351,52 @@ __device__ __forceinline__ int sum_up(const int *total, int *first, int experts)
   const int lane = threadIdx.x & 63;
   int before = 0;
   for (int e0 = 0; e0 < experts; e0 += 64) {
-    const int n = e0 + lane < experts ? total[e0 + lane] : 0;
-    int sum = n;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int t = __shfl_up(sum, d);
-      if (lane >= d) sum += t;
-    }
-    if (e0 + lane < experts) first[e0 + lane] = before + sum - n;
-    before += __shfl(sum, 63);
+    int all;
+    const int at = sum_before(e0 + lane < experts ? total[e0 + lane] : 0, &all);
+    if (e0 + lane < experts) first[e0 + lane] = before + at;
+    before += all;
   }
   return before;
 }
 
-__global__ __launch_bounds__(512) void k_route_place(RouteArgs a, int blocks)
+// The slots of a workgroup of k_route_choose in their places: four waves, each with a quarter of them, that count first
+__global__ __launch_bounds__(256) void k_route_place(RouteArgs a)
 {
-  __shared__ int total[1024], next[1024], first[1024], all;
-  for (int e = threadIdx.x; e < a.experts; e += 512) {
-    int sum = 0, before = 0;
-    for (int b = 0; b < blocks; ++b) {
-      const int n = a.hist[(long long)b * a.experts + e];
-      before += b < (int)blockIdx.x ? n : 0;
-      sum += n;
-    }
-    total[e] = sum;
-    next[e] = before;
+  __shared__ int first[1024], next[4][1024], all;
+  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+  const long long from = (long long)blockIdx.x * kRouteBlock * a.topk, end = a.tokens * a.topk;
+  const int count = (int)(end - from < (long long)kRouteBlock * a.topk ? end - from : (long long)kRouteBlock * a.topk);
+  const int quarter = (count + 255) / 256 * 64, mine = wave * quarter, to = mine + quarter < count ? mine + quarter : count;
+  for (int e = threadIdx.x; e < a.experts; e += 256) {
+    first[e] = a.totals[e];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) next[w][e] = 0;
   }
   __syncthreads();
-  if (threadIdx.x < 64) {
-    const int n = sum_up(total, first, a.experts);
-    if (threadIdx.x == 0) all = n;
+  for (int i = mine + lane; i < to; i += 64) {
+    const int id = a.ids[from + i];
+    if (id >= 0) atomicAdd(&next[wave][id], 1);
+  }
+  if (wave == 0) {
+    const int n = sum_up(first, first, a.experts);
+    if (lane == 0) all = n;
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < a.experts; e += 512) {
-    next[e] += first[e];
+  for (int e = threadIdx.x; e < a.experts; e += 256) {
     if (blockIdx.x == 0) a.offsets[e] = first[e];
+    int at = first[e] + a.hist[(long long)e * gridDim.x + blockIdx.x];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const int n = next[w][e];
+      next[w][e] = at;
+      at += n;
+    }
   }
   if (blockIdx.x == 0 && threadIdx.x == 0) a.offsets[a.experts] = all;
   __syncthreads();
-  const long long from = (long long)blockIdx.x * kRouteBlock * a.topk, end = a.tokens * a.topk;
-  const int count = (int)(end - from < (long long)kRouteBlock * a.topk ? end - from : (long long)kRouteBlock * a.topk);
-  if (threadIdx.x < 64) place(a, a.ids + from, from, count, next);
+  if (mine < to) place(a, a.ids + from + mine, from + mine, to - mine, next[wave]);
   // behind the last expert's: none.  Every workgroup has its share of the places that could be left
-  for (long long i = from + threadIdx.x; i < from + count; i += 512)
+  for (long long i = from + threadIdx.x; i < from + count; i += 256)
     if (i >= all) a.slots[i] = -1;
 }
 
@@ -241,15 +405,18 @@ template <int TYPE, int PER>
 __global__ __launch_bounds__(1024) void k_route_few(RouteArgs a)
 {
   constexpr int WAVES = 16;
-  __shared__ float keys[WAVES][64 * PER];
+  __shared__ float room[WAVES][64 * PER];
   __shared__ int count[64 * PER], next[64 * PER], ids[kRouteBlock * 32], all;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int e = threadIdx.x; e < a.experts; e += 1024) count[e] = 0;
   __syncthreads();
+  const Groups<PER> groups = groups_of<PER>(a);
   for (int t = wave; t < a.tokens; t += WAVES) {
     int id;
     float w;
-    choose<TYPE, PER>(a, t, keys[wave], &id, &w);
+    float x[PER];
+    load_logits<TYPE, PER>(a, t, x);
+    choose<PER>(a, groups, x, room[wave], &id, &w);
     if (lane < a.topk) {
       a.ids[t * a.topk + lane] = id;
       a.weights[t * a.topk + lane] = w;
@@ -281,8 +448,11 @@ hipError_t run(const RouteArgs &a, hipStream_t s)
     return hipGetLastError();
   }
   const unsigned blocks = (unsigned)((a.tokens + kRouteBlock - 1) / kRouteBlock);
-  hipLaunchKernelGGL((k_route_choose<TYPE, PER>), dim3(blocks), dim3(512), 0, s, a);
-  if (a.offsets) hipLaunchKernelGGL(k_route_place, dim3(blocks), dim3(512), 0, s, a, (int)blocks);
+  hipLaunchKernelGGL((k_route_choose<TYPE, PER>), dim3(blocks), dim3(1024), 0, s, a);
+  if (a.offsets) {
+    hipLaunchKernelGGL(k_route_sum, dim3((a.experts + 3) / 4), dim3(256), 0, s, a, (int)blocks);
+    hipLaunchKernelGGL(k_route_place, dim3(blocks), dim3(256), 0, s, a);
+  }
   return hipGetLastError();
 }
 
