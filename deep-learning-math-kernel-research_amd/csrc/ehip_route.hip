@@ -7,6 +7,8 @@
 // 21 (32768 tokens, 256 experts in 8 groups, 8 choices).
 // The slots of an expert keep the order of the tokens: workgroups count theirs, a kernel sums the counts over the workgroups
 // before each, a third places the slots.  A few tokens take one workgroup and one launch.
+#include <type_traits>
+
 #include "ehip_layers.hpp"
 
 namespace ehip {
@@ -42,12 +44,13 @@ __device__ __forceinline__ int imin(int a, int b) { return a < b ? a : b; }
 // the maximum over the wave, in every lane (a scalar)
 __device__ __forceinline__ int max_over_wave(int v)
 {
-  v = imax(v, dpp<kShr1>(v, v));
-  v = imax(v, dpp<kShr2>(v, v));
-  v = imax(v, dpp<kShr4>(v, v));
-  v = imax(v, dpp<kShr8>(v, v));
-  v = imax(v, dpp<kBcast15, 0xa>(v, v));
-  v = imax(v, dpp<kBcast31, 0xc>(v, v));
+  constexpr int least = (int)0x80000000;   // (with it the step is one instruction)
+  v = imax(v, dpp<kShr1>(least, v));
+  v = imax(v, dpp<kShr2>(least, v));
+  v = imax(v, dpp<kShr4>(least, v));
+  v = imax(v, dpp<kShr8>(least, v));
+  v = imax(v, dpp<kBcast15, 0xa>(least, v));
+  v = imax(v, dpp<kBcast31, 0xc>(least, v));
   return __builtin_amdgcn_readlane(v, 63);
 }
 template <int CTRL, int ROWS = 0xf>
@@ -85,16 +88,17 @@ __device__ __forceinline__ void load_logits(const RouteArgs &a, long long token,
   for (int j = 0; j < PER; ++j) x[j] = first + j < a.experts ? load_one(row + j * size, TYPE) : kClosed;
 }
 
-// How the groups lie over a wave: 64 / (groups rounded up to a power of two) lanes look through one
-template <int PER> struct Groups {
+// What is the same for every token: the bias of the lane's experts (0 where there is none), and how the groups lie over a wave: 64 / (groups rounded up to a power of two) lanes look through one
+template <int PER> struct Fixed {
+  float bias[PER];
   int size, lanes, mine;
   bool own;             // each lane's keys are of the group that it looks through
   unsigned char at[PER];   // lane that speaks for the group of each of the lane's experts
 };
 template <int PER>
-__device__ __forceinline__ Groups<PER> groups_of(const RouteArgs &a)
+__device__ __forceinline__ Fixed<PER> fixed_of(const RouteArgs &a)
 {
-  Groups<PER> g;
+  Fixed<PER> g;
   const int lane = threadIdx.x & 63;
   g.size = a.experts / a.groups;
   g.lanes = 64;
@@ -104,6 +108,7 @@ __device__ __forceinline__ Groups<PER> groups_of(const RouteArgs &a)
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     const int e = lane * PER + j;
+    g.bias[j] = a.bias && e < a.experts ? a.bias[e] : 0.0f;
     g.at[j] = (unsigned char)(e < a.experts ? e / g.size * g.lanes : 0);
   }
   return g;
@@ -118,15 +123,15 @@ __device__ __forceinline__ void join(int &b1, int &b2, int o1, int o2)
 
 // One token from its logits: lane j < topk returns its j-th choice (-1: none) and that choice's weight.  room: of the wave
 template <int PER>
-__device__ __forceinline__ void choose(const RouteArgs &a, const Groups<PER> &g, float (&x)[PER], float *room, int *id_out, float *weight_out)
+__device__ __forceinline__ void choose(const RouteArgs &a, const Fixed<PER> &g, float (&x)[PER], float *room, int *id_out, float *weight_out)
 {
   const int lane = threadIdx.x & 63, first = lane * PER;
   float score[PER];
   int key[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    x[j] = x[j] > kClosed ? x[j] : kClosed;   // a NaN is closed, too
-    x[j] = x[j] < 3.402823466e38f ? x[j] : 3.402823466e38f;
+    x[j] = x[j] > kClosed ? +x[j] : kClosed;   // a NaN is closed, too
+    x[j] = x[j] < 3.402823466e38f ? +x[j] : 3.402823466e38f;
   }
   if (a.sigmoid) {
 #pragma unroll
@@ -148,8 +153,7 @@ __device__ __forceinline__ void choose(const RouteArgs &a, const Groups<PER> &g,
   }
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
-    float k = score[j];
-    if (a.bias && first + j < a.experts) k += a.bias[first + j];
+    const float k = score[j] + g.bias[j];
     key[j] = x[j] > kClosed && k == k ? ordered(k) : kClosedKey;
   }
 
@@ -191,36 +195,39 @@ __device__ __forceinline__ void choose(const RouteArgs &a, const Groups<PER> &g,
   for (int j = 0; j < PER; ++j) room[first + j] = score[j];
 
   // exchanges of neighbours only, of unequal keys only: equal ones stay in the order of their experts
-  int expert[PER];
+  int from[PER];
 #pragma unroll
-  for (int j = 0; j < PER; ++j) expert[j] = first + j;
+  for (int j = 0; j < PER; ++j) from[j] = j;
 #pragma unroll
   for (int i = 0; i < PER - 1; ++i)
 #pragma unroll
     for (int j = PER - 2; j >= i; --j) {
       const bool swap = key[j + 1] > key[j];
-      const int k = key[j];
-      const int e = expert[j];
-      key[j] = swap ? key[j + 1] : k;
-      expert[j] = swap ? expert[j + 1] : e;
-      key[j + 1] = swap ? k : key[j + 1];
-      expert[j + 1] = swap ? e : expert[j + 1];
+      const int k = imin(key[j], key[j + 1]), f = from[j];
+      key[j] = imax(key[j], key[j + 1]);
+      key[j + 1] = k;
+      const int f1 = from[j + 1];
+      from[j] = swap ? +f1 : +f;   // (values: a choice between array elements would make them memory)
+      from[j + 1] = swap ? +f : +f1;
     }
+  // the order as 4 bits an expert
+  typedef typename std::conditional<(PER > 8), uint64_t, uint32_t>::type Order;
+  Order order = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) order |= (Order)from[j] << (4 * j);
 
   int id = -1;
   for (int k = 0; k < a.topk; ++k) {
     const int m = max_over_wave(key[0]);
     if (m == kClosedKey) break;
     const int who = __builtin_ctzll(__ballot(key[0] == m));
-    const int e = __builtin_amdgcn_readlane(expert[0], who);
+    const int e = who * PER + __builtin_amdgcn_readlane((int)(order & 15), who);
     id = lane == k ? e : id;
     const bool mine = lane == who;
 #pragma unroll
-    for (int j = 0; j + 1 < PER; ++j) {
-      key[j] = mine ? key[j + 1] : key[j];
-      expert[j] = mine ? expert[j + 1] : expert[j];
-    }
-    key[PER - 1] = mine ? kClosedKey : key[PER - 1];
+    for (int j = 0; j + 1 < PER; ++j) key[j] = mine ? +key[j + 1] : +key[j];
+    key[PER - 1] = mine ? kClosedKey : +key[PER - 1];
+    order = mine ? order >> 4 : order;
   }
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   float weight = id >= 0 ? room[id] : 0.0f;
@@ -251,21 +258,25 @@ __global__ __launch_bounds__(1024) void k_route_choose(RouteArgs a)
   for (int e = threadIdx.x; e < a.experts; e += 64 * WAVES) count[e] = 0;
   __syncthreads();
   const long long from = (long long)blockIdx.x * kRouteBlock, to = from + kRouteBlock < a.tokens ? from + kRouteBlock : a.tokens;
-  const Groups<PER> groups = groups_of<PER>(a);
+  const Fixed<PER> fixed = fixed_of<PER>(a);
   float x[PER], ahead[PER];
   if (from + wave < to) load_logits<TYPE, PER>(a, from + wave, ahead);
+  int32_t *ids = a.ids + (from + wave) * a.topk + lane;
+  float *weights = a.weights + (from + wave) * a.topk + lane;
   for (long long t = from + wave; t < to; t += WAVES) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) x[j] = ahead[j];
     if (t + WAVES < to) load_logits<TYPE, PER>(a, t + WAVES, ahead);
     int id;
     float w;
-    choose<PER>(a, groups, x, room[wave], &id, &w);
+    choose<PER>(a, fixed, x, room[wave], &id, &w);
     if (lane < a.topk) {
-      a.ids[t * a.topk + lane] = id;
-      a.weights[t * a.topk + lane] = w;
+      *ids = id;
+      *weights = w;
       if (id >= 0) atomicAdd(&count[id], 1);
     }
+    ids += WAVES * a.topk;
+    weights += WAVES * a.topk;
   }
   if (!a.hist) return;
   __syncthreads();
@@ -410,13 +421,13 @@ __global__ __launch_bounds__(1024) void k_route_few(RouteArgs a)
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   for (int e = threadIdx.x; e < a.experts; e += 1024) count[e] = 0;
   __syncthreads();
-  const Groups<PER> groups = groups_of<PER>(a);
+  const Fixed<PER> fixed = fixed_of<PER>(a);
   for (int t = wave; t < a.tokens; t += WAVES) {
     int id;
     float w;
     float x[PER];
     load_logits<TYPE, PER>(a, t, x);
-    choose<PER>(a, groups, x, room[wave], &id, &w);
+    choose<PER>(a, fixed, x, room[wave], &id, &w);
     if (lane < a.topk) {
       a.ids[t * a.topk + lane] = id;
       a.weights[t * a.topk + lane] = w;
