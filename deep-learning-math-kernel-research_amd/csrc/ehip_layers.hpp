@@ -37,6 +37,7 @@ struct LinearArgs {
   int experts, topk, in_rows, out_rows;
   int out_type, act, gated;
   float res_scale;
+  int form;                 // EHIP_LINEAR_FORM, or -1
   int blocks_m, blocks_n;   // set by the launcher
 };
 

@@ -10,6 +10,7 @@ using namespace ehip;
 struct ehip_linear {
   ehip_linear_desc_t d;
   int elem = 0, tiles = 0, chunks = 0;
+  int form = -1;   // EHIP_LINEAR_FORM: forces a kernel form (a gated product needs one with an even number of tiles)
   char *packed = nullptr;   // weights, and behind them the scales, the bias and 256 bytes of zeros
   float *scale = nullptr, *bias = nullptr;
   char *zeros = nullptr;
@@ -115,6 +116,7 @@ int linear_args(const ehip_linear *h, const ehip_linear_args_t &g, LinearArgs *a
   a->act = d.activation;
   a->gated = d.gated;
   a->res_scale = d.residual_scale;
+  a->form = h->form;
   return EHIP_OK;
 }
 
@@ -133,6 +135,7 @@ EHIP_API int ehip_linear_create(const ehip_linear_desc_t *desc, ehip_linear_t **
     if (!h) return fail(EHIP_GENERAL_ERROR, "out of host memory");
     h->d = *desc;
     h->elem = size_of(desc->input_type);
+    if (const char *env = getenv("EHIP_LINEAR_FORM")) h->form = atoi(env);
     h->tiles = desc->gated ? (desc->oc + 31) / 32 * 4 : (desc->oc + 63) / 64 * 4;
     h->chunks = (int)(((int64_t)desc->ic * h->elem + 127) / 128 * 2);
     const size_t blocks = (size_t)desc->experts * h->tiles * h->chunks, constants = (size_t)desc->experts * h->tiles * 16 * 4;
@@ -231,6 +234,7 @@ EHIP_API const char *ehip_linear_kernel_name(const ehip_linear_t *h, int64_t row
   a.chunks = h->chunks;
   a.gated = h->d.gated;
   a.experts = h->d.experts;
+  a.form = h->form;
   static const int32_t none = 0;
   if (h->d.experts > 1) a.offsets = &none;   // (only whether there are any is asked)
   return linear_kernel_name(a, h->d.input_type);

@@ -62,39 +62,47 @@ hipError_t launch_linear_constants(float *dst, const float *src, int experts, in
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------------------
-// A workgroup has NT tiles of 16 weights rows x MT tiles of 16 activations rows; its waves share K out in runs of chunks, so
-// no operand is read twice and the weights stream past as runs of KBs.  U chunks are in flight while U are multiplied.  The
+// A workgroup has NT tiles of 16 weights rows x MT tiles of 16 activations rows; its waves share K out in runs of steps of 128
+// bytes, so no weight is read twice and they stream past as runs of KBs, straight into registers, P steps ahead.  Activations
+// come by whole lines, 8 lanes a row, and change lanes through a corner of LDS that is the wave's own (a load that gave every
+// lane the 16 bytes that its matrix operand has would be 64 accesses instead of 16, and the loads bound these kernels).  The
 // waves' sums meet in LDS, in the order of the waves.
-template <int TYPE, int NT, int MT, int WAVES, int U>
-__global__ __launch_bounds__(WAVES * 64) void k_linear_split(LinearArgs a)
+template <int TYPE, int NT, int MT, int P>
+__global__ __launch_bounds__(512) void k_linear_split(LinearArgs a)
 {
-  typedef Product<TYPE> P;
-  typedef typename P::Acc Acc;
-  __shared__ Acc red[WAVES][NT * MT][64];
+  typedef Product<TYPE> Pr;
+  typedef typename Pr::Acc Acc;
+  constexpr int WAVES = 8;
+  constexpr int ROOM = MT * 2048 > NT * MT * 1024 ? MT * 2048 : NT * MT * 1024;   // bytes of LDS a wave
+  __shared__ i4 lds[WAVES * ROOM / 16];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, c = lane & 15;
 
   // blocks of the same weights beside each other on one XCD: its L2 holds them for all
   const int per_xcd = (a.blocks_m * a.blocks_n + 7) / 8;
   const int index = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-  if (index >= a.blocks_m * a.blocks_n) return;
+  if ((int)(blockIdx.x >> 3) >= per_xcd || index >= a.blocks_m * a.blocks_n) return;
   const int bn = index / a.blocks_m;
   const Block blk = block_of(a, index - bn * a.blocks_m, 16 * MT);
   if (blk.expert < 0) return;
 
-  const char *xp[MT];
+  // the 16-byte part of row r that a lane loads changes places by r % 8: the 8 rows that are read at a time lie in different banks
+  const int part = (lane & 7) ^ (lane >> 3);
+  const char *xp[2 * MT];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const long long p = blk.first + m * 16 + c;
-    xp[m] = a.x + row_of(a, p < blk.last ? p : blk.last - 1).in * a.ldx + g * 16;
+  for (int i = 0; i < 2 * MT; ++i) {
+    const long long p = blk.first + i * 8 + (lane >> 3);
+    xp[i] = a.x + row_of(a, p < blk.last ? p : blk.last - 1).in * a.ldx + part * 16;
   }
   const int tile0 = bn * NT;
   const long long tile_bytes = (long long)a.chunks * 1024;
   const char *wp = a.w + ((long long)blk.expert * a.tiles + tile0) * tile_bytes;
   const unsigned wl = lane * 16;
+  i4 *own = lds + wave * (ROOM / 16);
+  const int xread = c * 8 + (g ^ (c & 7));   // (of the second half: the same, 4 parts away)
 
-  const int full = a.kbytes >> 6;
-  const int per = (full + WAVES - 1) / WAVES, c0 = wave * per, c1 = c0 + per < full ? c0 + per : full;
+  const int full = a.kbytes >> 7, per = (full + WAVES - 1) / WAVES;
+  const int k0 = wave * per, k1 = k0 + per < full ? k0 + per : full;
 
   Acc acc[NT][MT];
 #pragma unroll
@@ -102,55 +110,68 @@ __global__ __launch_bounds__(WAVES * 64) void k_linear_split(LinearArgs a)
 #pragma unroll
     for (int m = 0; m < MT; ++m) acc[n][m] = Acc{0, 0, 0, 0};
 
-  auto load = [&](i4 (&wq)[U][NT], i4 (&xq)[U][MT], int at) {
+  i4 wr[P][2 * NT], xr[P][2 * MT];
+  auto load = [&](int slot, int k) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int k = at + u < c1 ? at + u : c1 - 1;
+    for (int n = 0; n < 2 * NT; ++n)
+      wr[slot][n] = *reinterpret_cast<const i4 *>(wp + (n >> 1) * tile_bytes + (long long)k * 2048 + (n & 1) * 1024 + wl);
 #pragma unroll
-      for (int n = 0; n < NT; ++n) wq[u][n] = *reinterpret_cast<const i4 *>(wp + n * tile_bytes + (long long)k * 1024 + wl);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) xq[u][m] = *reinterpret_cast<const i4u *>(xp[m] + (long long)k * 64);
-    }
+    for (int i = 0; i < 2 * MT; ++i) xr[slot][i] = *reinterpret_cast<const i4u *>(xp[i] + (long long)k * 128);
+    __builtin_amdgcn_sched_barrier(0);   // (loads stay behind the products that free their registers)
   };
-  auto multiply = [&](i4 (&wq)[U][NT], i4 (&xq)[U][MT], int count) {
+  auto multiply = [&](const i4 (&w)[2 * NT], const i4 (&x)[2 * MT]) {
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (u < count) {
+    for (int i = 0; i < 2 * MT; ++i) own[i * 64 + lane] = x[i];
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+    for (int h = 0; h < 2; ++h) {
+      i4 xq[MT];
 #pragma unroll
-          for (int m = 0; m < MT; ++m) acc[n][m] = P::mma(wq[u][n], xq[u][m], acc[n][m]);
+      for (int m = 0; m < MT; ++m) xq[m] = own[m * 128 + (xread ^ (h * 4))];
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int m = 0; m < MT; ++m) acc[n][m] = Pr::mma(w[2 * n + h], xq[m], acc[n][m]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (k0 < k1) {
+    // steps past the wave's last repeat it (they come from cache, and nobody waits for them)
+#pragma unroll
+    for (int s = 0; s < P; ++s) load(s, k0 + s < k1 ? k0 + s : k1 - 1);
+    int k = k0;
+    for (; k + P < k1; k += P)
+#pragma unroll
+      for (int s = 0; s < P; ++s) {
+        multiply(wr[s], xr[s]);
+        load(s, k + s + P < k1 ? k + s + P : k1 - 1);
       }
-  };
-  i4 w0[U][NT], x0[U][MT], w1[U][NT], x1[U][MT];
-  if (c0 < c1) load(w0, x0, c0);
-  if (wave == WAVES - 1 && (a.kbytes & 63)) {   // the last chunk, of which a part exists
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const i4 w = *reinterpret_cast<const i4 *>(wp + n * tile_bytes + (long long)full * 1024 + wl);
-#pragma unroll
-      for (int m = 0; m < MT; ++m) acc[n][m] = P::mma(w, load_part<P::elem>(xp[m] + (long long)full * 64, (a.kbytes & 63) - g * 16), acc[n][m]);
-    }
+    for (int s = 0; s < P; ++s)
+      if (k + s < k1) multiply(wr[s], xr[s]);
   }
-  for (int k = c0; k < c1; k += 2 * U) {
-    if (k + U < c1) load(w1, x1, k + U);
-    multiply(w0, x0, c1 - k);
-    if (k + U < c1) {
-      if (k + 2 * U < c1) load(w0, x0, k + 2 * U);
-      multiply(w1, x1, c1 - k - U);
-    }
+  if (wave == WAVES - 1 && (a.kbytes & 127)) {   // the last step, of which a part exists
+    i4 w[2 * NT], x[2 * MT];
+#pragma unroll
+    for (int n = 0; n < 2 * NT; ++n)
+      w[n] = *reinterpret_cast<const i4 *>(wp + (n >> 1) * tile_bytes + (long long)full * 2048 + (n & 1) * 1024 + wl);
+#pragma unroll
+    for (int i = 0; i < 2 * MT; ++i) x[i] = load_part<Pr::elem>(xp[i] + (long long)full * 128, (a.kbytes & 127) - part * 16);
+    multiply(w, x);
   }
 
+  __syncthreads();
 #pragma unroll
   for (int n = 0; n < NT; ++n)
 #pragma unroll
-    for (int m = 0; m < MT; ++m) red[wave][n * MT + m][lane] = acc[n][m];
+    for (int m = 0; m < MT; ++m) own[(n * MT + m) * 64 + lane] = __builtin_bit_cast(i4, acc[n][m]);
   __syncthreads();
 
   auto total = [&](int n, int m) {
-    Acc s = red[0][n * MT + m][lane];
+    Acc s = __builtin_bit_cast(Acc, lds[(n * MT + m) * 64 + lane]);
 #pragma unroll
-    for (int v = 1; v < WAVES; ++v) s += red[v][n * MT + m][lane];
+    for (int v = 1; v < WAVES; ++v) s += __builtin_bit_cast(Acc, lds[v * (ROOM / 16) + (n * MT + m) * 64 + lane]);
     return s;
   };
   constexpr int PAIRS = NT > 1 ? NT / 2 : 1;
@@ -195,21 +216,22 @@ long long blocks_of(const LinearArgs &a, int rows)
   return a.rows / rows + (a.rows < a.experts ? a.rows : a.experts);
 }
 
-template <int TYPE, int NT, int MT, int WAVES, int U>
+template <int TYPE, int NT, int MT, int P>
 hipError_t run_split(LinearArgs a, hipStream_t s)
 {
   const long long m = blocks_of(a, 16 * MT), n = a.tiles / NT, all = (m * n + 7) / 8 * 8;
   if (all >= 1ll << 31) return hipErrorInvalidValue;
   a.blocks_m = (int)m;
   a.blocks_n = (int)n;
-  hipLaunchKernelGGL((k_linear_split<TYPE, NT, MT, WAVES, U>), dim3((unsigned)all), dim3(WAVES * 64), 0, s, a);
+  hipLaunchKernelGGL((k_linear_split<TYPE, NT, MT, P>), dim3((unsigned)all), dim3(512), 0, s, a);
   return hipGetLastError();
 }
 
-enum Form { SPLIT_1X1, SPLIT_2X1, SPLIT_2X2, SPLIT_4X4, TILE_128, TILE_256 };
+enum Form { SPLIT_1X1, SPLIT_2X1, SPLIT_4X1, SPLIT_1X2, SPLIT_2X2, SPLIT_4X2, SPLIT_2X4, SPLIT_4X4, TILE_128, TILE_256, FORMS };
 
 Form choose(const LinearArgs &a)
 {
+  if (a.form >= 0 && a.form < FORMS && !(a.gated && (a.form == SPLIT_1X1 || a.form == SPLIT_1X2))) return (Form)a.form;
   const double rows = a.offsets ? (double)a.rows / a.experts : (double)a.rows;   // of one matrix
   if (rows > 192) return TILE_256;
   if (rows > 32) return SPLIT_4X4;
@@ -221,10 +243,14 @@ template <int TYPE>
 hipError_t launch_typed(const LinearArgs &a, hipStream_t s)
 {
   switch (choose(a)) {
-  case SPLIT_1X1: return run_split<TYPE, 1, 1, 8, 8>(a, s);
-  case SPLIT_2X1: return run_split<TYPE, 2, 1, 8, 6>(a, s);
-  case SPLIT_2X2: return run_split<TYPE, 2, 2, 8, 4>(a, s);
-  case SPLIT_4X4: return run_split<TYPE, 4, 4, 8, 2>(a, s);
+  case SPLIT_1X1: return run_split<TYPE, 1, 1, 4>(a, s);
+  case SPLIT_2X1: return run_split<TYPE, 2, 1, 4>(a, s);
+  case SPLIT_4X1: return run_split<TYPE, 4, 1, 3>(a, s);
+  case SPLIT_1X2: return run_split<TYPE, 1, 2, 4>(a, s);
+  case SPLIT_2X2: return run_split<TYPE, 2, 2, 3>(a, s);
+  case SPLIT_4X2: return run_split<TYPE, 4, 2, 2>(a, s);
+  case SPLIT_2X4: return run_split<TYPE, 2, 4, 2>(a, s);
+  case SPLIT_4X4: return run_split<TYPE, 4, 4, 2>(a, s);
   case TILE_128: return launch_linear_tile(a, TYPE, 0, blocks_of(a, 128), s);
   default: return launch_linear_tile(a, TYPE, 1, blocks_of(a, 256), s);
   }
@@ -243,8 +269,9 @@ hipError_t launch_linear(const LinearArgs &a, int type, hipStream_t s)
 
 const char *linear_kernel_name(const LinearArgs &a, int)
 {
-  static const char *const names[] = {"k_linear_split<1x1>", "k_linear_split<2x1>", "k_linear_split<2x2>", "k_linear_split<4x4>",
-                                      "k_linear_tile<128x128>", "k_linear_tile<256x256>"};
+  static const char *const names[FORMS] = {"k_linear_split<1x1>", "k_linear_split<2x1>", "k_linear_split<4x1>", "k_linear_split<1x2>",
+                                           "k_linear_split<2x2>", "k_linear_split<4x2>", "k_linear_split<2x4>", "k_linear_split<4x4>",
+                                           "k_linear_tile<128x128>", "k_linear_tile<256x256>"};
   return names[choose(a)];
 }
 
