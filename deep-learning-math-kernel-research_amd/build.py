@@ -71,9 +71,10 @@ EXTRA_FLAGS = {
     "ehip_fewch.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "ehip_gemm1x1s.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
     "ehip_gemm1x1w.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16", "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-    # a tile kernel's epilogue indexes its accumulators by constants only where it is unrolled whole; m0, which its loads into
-    # LDS set, is a register that the compiler keeps to itself
-    "ehip_linear_tile.hip": ["-mllvm", "-pragma-unroll-threshold=1000000", "-Wno-inline-asm"],
+    # the 128 x 128 form's accumulators: in the accumulation registers half of them would be moved around each product.  m0, which
+    # the loads into LDS set, is a register that the compiler keeps to itself
+    "ehip_linear_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-pragma-unroll-threshold=1000000", "-Wno-inline-asm"],
+    "ehip_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     # and those of the 1x1 kernels with few input channels
     "ehip_gemm.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],
 }

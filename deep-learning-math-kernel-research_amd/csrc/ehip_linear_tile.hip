@@ -11,13 +11,13 @@ __device__ __forceinline__ void load_to_lds(const char *src, unsigned lds)
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "m0");
 }
 
-// A workgroup has WN x WM waves of NTW x MTW tiles of 16 x 16 results.  A step is 128 bytes of K, in two halves; LDS holds two
-// steps.  A wave multiplies one half out of registers while it reads the next into others.  The workgroup meets once a step,
-// between the halves: by then every wave has read the whole step, and the next one has arrived; the one after it is loaded
-// into the place that came free.
+// A workgroup has WN x WM waves of NTW x MTW tiles of 16 x 16 results.  A step is 128 bytes of K, in two halves.  A wave multiplies one half out of registers while it reads the next into others.  The workgroup meets once a step,
+// between the halves: by then every wave has read the whole step, and the next one has arrived; another one is loaded into the
+// place that came free.  LDS holds STAGES steps: with two, a step's loads have the time of one step, which 256 x 256 results
+// cover; 128 x 128 do not, and take four.
 // ALIGNED: rows of activations at multiples of 16 bytes and a whole number of 16-byte parts in K, so they go straight into LDS
 // like the weights; else through registers.
-template <int TYPE, int NTW, int MTW, int WN, int WM, bool ALIGNED>
+template <int TYPE, int NTW, int MTW, int WN, int WM, int STAGES, bool ALIGNED>
 __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
 {
   typedef Product<TYPE> P;
@@ -106,52 +106,53 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
       if (loads) {
 #pragma unroll
         for (int j = 0; j < PER; ++j)
-          if (n * PER + j < LOADS) load(n * PER + j, step, step & 1);
+          if (n * PER + j < LOADS) load(n * PER + j, step, step % STAGES);
       }
-      read(2 * n, from & 1, h ^ 1);
-      read(2 * n + 1, from & 1, h ^ 1);
+      read(2 * n, from % STAGES, h ^ 1);
+      read(2 * n + 1, from % STAGES, h ^ 1);
 #pragma unroll
       for (int m = 0; m < MTW; ++m) acc[n][m] = P::mma(wq[h][n], xq[h][m], acc[n][m]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  auto meet = [&]() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" : : : "memory");
+  // every wave is done with what came before, and all of its loads but the youngest `flying` have arrived
+  auto meet = [&](auto flying) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" : : "n"(flying.value) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" : : : "memory");
   };
 
+  static_assert(ALIGNED || STAGES == 2, "through registers, a step is a stage ahead");
 #pragma unroll
-  for (int j = 0; j < LOADS; ++j) load(j, 0, 0);
-  fetch(0);
-  put(0);
-  if (steps > 1) {
+  for (int st = 0; st < STAGES; ++st)
+    if (st < steps) {
 #pragma unroll
-    for (int j = 0; j < LOADS; ++j) load(j, 1, 1);
-    fetch(1);
-    put(1);
-  }
-  meet();
+      for (int j = 0; j < LOADS; ++j) load(j, st, st);
+      fetch(st);
+      put(st);
+    }
+  if (steps >= STAGES) meet(Const<(STAGES - 1) * LOADS * ALIGNED>());
+  else meet(Const<0>());
 #pragma unroll
   for (int j = 0; j < MTW + NTW; ++j) read(j, 0, 0);
   int step = 0;
-  for (; step + 2 < steps; ++step) {
-    fetch(step + 2);
+  for (; step + STAGES < steps; ++step) {
+    fetch(step + STAGES);
     half(0, step, 0, false);
-    meet();
-    put(step & 1);
-    half(1, step + 1, step + 2, true);
+    meet(Const<(STAGES - 2) * LOADS>());
+    put(step % STAGES);
+    half(1, step + 1, step + STAGES, true);
   }
   for (; step < steps; ++step) {
     half(0, step, 0, false);
-    meet();
+    meet(Const<0>());
     half(1, step + 1, 0, false);
   }
 
   // The results go through LDS, 16 rows of every wave at a time, and come back as runs of 8 columns a thread: a wave then has
   // whole rows of results beside each other in memory.
   constexpr int ROW = BN * 64 + 16, THREADS = WAVES * 64;   // bytes of a row: its last 16 keep rows off each other's banks
-  static_assert(WM * 16 * ROW <= 2 * STAGE, "16 rows of every wave fit");
+  static_assert(WM * 16 * ROW <= STAGES * STAGE, "16 rows of every wave fit");
   for_epilogue(a, [&](auto act, auto type, auto gated) {
     constexpr bool GATED = gated.value;
     constexpr int SIZE = type.value == EHIP_F32 ? 4 : 2;
@@ -225,7 +226,7 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
 
 namespace {
 
-template <int TYPE, int NTW, int MTW, int WN, int WM>
+template <int TYPE, int NTW, int MTW, int WN, int WM, int STAGES>
 hipError_t run(LinearArgs a, long long blocks_m, hipStream_t s)
 {
   const long long n = (a.tiles + NTW * WN - 1) / (NTW * WN), all = (blocks_m * n + 7) / 8 * 8;
@@ -233,8 +234,8 @@ hipError_t run(LinearArgs a, long long blocks_m, hipStream_t s)
   a.blocks_m = (int)blocks_m;
   a.blocks_n = (int)n;
   const bool aligned = ((uintptr_t)a.x | (unsigned long long)a.ldx | (unsigned)a.kbytes) % 16 == 0;
-  constexpr int lds = (NTW * WN + MTW * WM) * 2048 * 2;
-  auto kernel = aligned ? k_linear_tile<TYPE, NTW, MTW, WN, WM, true> : k_linear_tile<TYPE, NTW, MTW, WN, WM, false>;
+  const int lds = (NTW * WN + MTW * WM) * 2048 * (aligned ? STAGES : 2);
+  auto kernel = aligned ? k_linear_tile<TYPE, NTW, MTW, WN, WM, STAGES, true> : k_linear_tile<TYPE, NTW, MTW, WN, WM, 2, false>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(WN * WM * 64), lds, s, a);
@@ -244,8 +245,8 @@ hipError_t run(LinearArgs a, long long blocks_m, hipStream_t s)
 template <int TYPE>
 hipError_t run_typed(const LinearArgs &a, int form, long long blocks_m, hipStream_t s)
 {
-  if (form == 0) return run<TYPE, 4, 4, 2, 2>(a, blocks_m, s);
-  return run<TYPE, 8, 4, 2, 4>(a, blocks_m, s);
+  if (form == 0) return run<TYPE, 4, 4, 2, 2, 4>(a, blocks_m, s);
+  return run<TYPE, 8, 4, 2, 4, 2>(a, blocks_m, s);
 }
 
 }  // namespace
