@@ -227,16 +227,66 @@ hipError_t run_split(LinearArgs a, hipStream_t s)
   return hipGetLastError();
 }
 
-enum Form { SPLIT_1X1, SPLIT_2X1, SPLIT_4X1, SPLIT_1X2, SPLIT_2X2, SPLIT_4X2, SPLIT_2X4, SPLIT_4X4, TILE_128, TILE_256, FORMS };
+enum Form { SPLIT_1X1, SPLIT_2X1, SPLIT_4X1, SPLIT_2X2, SPLIT_4X2, SPLIT_4X4, TILE_128, TILE_128_DEEP, TILE_256, FORMS };
+
+// What a form takes, in us, from what it measured on an idle card (bf16, f16 and s8 alike: a step is 128 bytes of K, and so are
+// its loads and its matrix instructions).  All forms: no faster than the bytes at 5.2 TB/s; what is hidden behind those is
+// not hidden whole.  Sweeps of 1 - 4096 rows, K 512 -
+// 8192 bytes, 1024 - 8192 columns, and of experts with 1 - 770 rows each: the form with the least sum is the fastest one or
+// within 15 % of it, in the worst case found 30 % (20 rows, 4096 x 4096: 9.8 us for 8.0).
+struct FormCost {
+  int nt, mt;          // tiles of a workgroup's results
+  int resident;        // workgroups of a CU
+  double start, round, step;   // once; for each time that the workgroups fill the card; for a step of one workgroup of a CU
+};
+constexpr FormCost kForms[FORMS] = {
+    // few rows: 0.019 us a tile of operands and step, which is what its loads take a CU (16 cycles a KB)
+    {1, 1, 2, 1.5, 1.2, 0.038}, {2, 1, 2, 1.5, 1.7, 0.057}, {4, 1, 1, 1.5, 2.1, 0.095}, {2, 2, 1, 1.5, 2.1, 0.076},
+    {4, 2, 1, 1.5, 2.4, 0.114}, {4, 4, 1, 1.5, 3.9, 0.17},
+    // 128 x 128: two workgroups of a CU with two steps in LDS (64 steps of 512 workgroups 64 us, of 256 42), or one with four (35)
+    {8, 8, 2, 0.0, 5.0, 0.47}, {8, 8, 1, 0.0, 5.0, 0.47},
+    // 256 x 256: 64 steps of 256 workgroups 101 us, of 128 76 (the clock is higher)
+    {16, 16, 1, 0.0, 10.0, 1.42}};
+
+double cost(const LinearArgs &a, Form form)
+{
+  const FormCost &f = kForms[form];
+  const double rows = (double)a.rows, high = 16.0 * f.mt, n = (a.tiles + f.nt - 1) / f.nt, steps = (a.kbytes + 127) / 128;
+  double m = (double)((a.rows + 16 * f.mt - 1) / (16 * f.mt)), matrices = 1;
+  if (a.offsets) {   // each expert's last block is half empty
+    matrices = rows < a.experts ? rows : a.experts;
+    const double each = rows / matrices / high + 0.5;
+    m = matrices * (each > 1 ? each : 1);
+  }
+  const double groups = m * n, fill = 256.0 * f.resident;
+  const double bytes = matrices * a.tiles * 16.0 * a.kbytes + rows * (a.kbytes + a.oc * (a.out_type == EHIP_F32 ? 4.0 : 2.0) * (a.res ? 2 : 1));
+  const double memory = bytes / 5.2e6;
+  double work;
+  if (form < TILE_128) {
+    work = (double)(long long)((groups + 255) / 256) * steps * f.step;
+    return f.start + (double)(long long)((groups + fill - 1) / fill) * f.round + (work > memory ? work + 0.3 * memory : memory + 0.3 * work);
+  }
+  const double whole = (double)(long long)(groups / fill), left = groups - whole * fill;
+  if (form == TILE_256) work = whole * (f.round + f.step * steps) + (left > 0 ? f.round + (1.0 + 0.42 * left / fill) * steps : 0);
+  else if (form == TILE_128) work = whole * (f.round + 2 * f.step * steps) + (left > 0 ? f.round + (left > 256 ? 2 * f.step : 0.58) * steps : 0);
+  else work = (whole + (left > 0)) * (f.round + f.step * steps);
+  return work > 1.2 * memory + f.round ? work : 1.2 * memory + f.round;
+}
 
 Form choose(const LinearArgs &a)
 {
-  if (a.form >= 0 && a.form < FORMS && !(a.gated && (a.form == SPLIT_1X1 || a.form == SPLIT_1X2))) return (Form)a.form;
-  const double rows = a.offsets ? (double)a.rows / a.experts : (double)a.rows;   // of one matrix
-  if (rows > 192) return TILE_256;
-  if (rows > 32) return SPLIT_4X4;
-  if (rows > 16) return SPLIT_2X2;
-  return a.gated ? SPLIT_2X1 : SPLIT_1X1;
+  const bool odd = a.gated;   // a gate and its partner are two tiles
+  if (a.form >= 0 && a.form < FORMS && !(odd && a.form == SPLIT_1X1)) return (Form)a.form;
+  int best = odd ? SPLIT_2X1 : SPLIT_1X1;
+  double least = cost(a, (Form)best);
+  for (int f = best + 1; f < FORMS; ++f) {
+    const double c = cost(a, (Form)f);
+    if (c < least) {
+      least = c;
+      best = f;
+    }
+  }
+  return (Form)best;
 }
 
 template <int TYPE>
@@ -246,13 +296,12 @@ hipError_t launch_typed(const LinearArgs &a, hipStream_t s)
   case SPLIT_1X1: return run_split<TYPE, 1, 1, 4>(a, s);
   case SPLIT_2X1: return run_split<TYPE, 2, 1, 4>(a, s);
   case SPLIT_4X1: return run_split<TYPE, 4, 1, 3>(a, s);
-  case SPLIT_1X2: return run_split<TYPE, 1, 2, 4>(a, s);
   case SPLIT_2X2: return run_split<TYPE, 2, 2, 3>(a, s);
   case SPLIT_4X2: return run_split<TYPE, 4, 2, 2>(a, s);
-  case SPLIT_2X4: return run_split<TYPE, 2, 4, 2>(a, s);
   case SPLIT_4X4: return run_split<TYPE, 4, 4, 2>(a, s);
   case TILE_128: return launch_linear_tile(a, TYPE, 0, blocks_of(a, 128), s);
-  default: return launch_linear_tile(a, TYPE, 1, blocks_of(a, 256), s);
+  case TILE_128_DEEP: return launch_linear_tile(a, TYPE, 1, blocks_of(a, 128), s);
+  default: return launch_linear_tile(a, TYPE, 2, blocks_of(a, 256), s);
   }
 }
 
@@ -269,9 +318,9 @@ hipError_t launch_linear(const LinearArgs &a, int type, hipStream_t s)
 
 const char *linear_kernel_name(const LinearArgs &a, int)
 {
-  static const char *const names[FORMS] = {"k_linear_split<1x1>", "k_linear_split<2x1>", "k_linear_split<4x1>", "k_linear_split<1x2>",
-                                           "k_linear_split<2x2>", "k_linear_split<4x2>", "k_linear_split<2x4>", "k_linear_split<4x4>",
-                                           "k_linear_tile<128x128>", "k_linear_tile<256x256>"};
+  static const char *const names[FORMS] = {"k_linear_split<1x1>", "k_linear_split<2x1>", "k_linear_split<4x1>", "k_linear_split<2x2>",
+                                           "k_linear_split<4x2>", "k_linear_split<4x4>", "k_linear_tile<128x128>",
+                                           "k_linear_tile<128x128, deep>", "k_linear_tile<256x256>"};
   return names[choose(a)];
 }
 

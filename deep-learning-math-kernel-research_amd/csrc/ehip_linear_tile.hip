@@ -13,8 +13,7 @@ __device__ __forceinline__ void load_to_lds(const char *src, unsigned lds)
 
 // A workgroup has WN x WM waves of NTW x MTW tiles of 16 x 16 results.  A step is 128 bytes of K, in two halves.  A wave multiplies one half out of registers while it reads the next into others.  The workgroup meets once a step,
 // between the halves: by then every wave has read the whole step, and the next one has arrived; another one is loaded into the
-// place that came free.  LDS holds STAGES steps: with two, a step's loads have the time of one step, which 256 x 256 results
-// cover; 128 x 128 do not, and take four.
+// place that came free.  LDS holds STAGES steps.
 // ALIGNED: rows of activations at multiples of 16 bytes and a whole number of 16-byte parts in K, so they go straight into LDS
 // like the weights; else through registers.
 template <int TYPE, int NTW, int MTW, int WN, int WM, int STAGES, bool ALIGNED>
@@ -245,7 +244,8 @@ hipError_t run(LinearArgs a, long long blocks_m, hipStream_t s)
 template <int TYPE>
 hipError_t run_typed(const LinearArgs &a, int form, long long blocks_m, hipStream_t s)
 {
-  if (form == 0) return run<TYPE, 4, 4, 2, 2, 4>(a, blocks_m, s);
+  if (form == 0) return run<TYPE, 4, 4, 2, 2, 2>(a, blocks_m, s);
+  if (form == 1) return run<TYPE, 4, 4, 2, 2, 4>(a, blocks_m, s);
   return run<TYPE, 8, 4, 2, 4, 2>(a, blocks_m, s);
 }
 
