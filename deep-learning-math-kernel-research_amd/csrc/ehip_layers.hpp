@@ -113,6 +113,19 @@ __device__ __forceinline__ void store_one(char *p, int type, float v)
   else *reinterpret_cast<__bf16 *>(p) = (__bf16)v;
 }
 
+// v of the lane that DPP control CTRL names; lanes without one, or outside of ROWS, keep `old`
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ int dpp(int old, int v)
+{
+  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float old, float v)
+{
+  return __builtin_bit_cast(float, dpp<CTRL, ROWS>(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v)));
+}
+constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143;
+
 // 16 bytes at p of which the first `valid` exist; the others are zero.  ELEM: bytes of an element
 template <int ELEM>
 __device__ __forceinline__ i4 load_part(const char *p, int valid)

@@ -1,5 +1,6 @@
 // The norm after a block, its gate and residual scale, and the norm before the next block, on rows held in registers: every
-// input is read once and every output written once, so memory bounds it.
+// input is read once and every output written once, so memory bounds it: 16384 x 4096 bf16 with both norms, gate and residual
+// 113 us, 4.77 TB/s of reads and writes (a large copy: 4.94).
 #include "ehip_layers.hpp"
 
 namespace ehip {
@@ -56,13 +57,34 @@ __device__ __forceinline__ void store8(char *p, int n, const float (&v)[8])
     if (j < n) store_one(p + j * Elem<TYPE>::size, TYPE, v[j]);
 }
 
+// over the 64 lanes, by cross-lane operands; the same bits in each of them
+__device__ __forceinline__ float over_wave(float v)
+{
+  v += dpp<kShr1>(0.0f, v);
+  v += dpp<kShr2>(0.0f, v);
+  v += dpp<kShr4>(0.0f, v);
+  v += dpp<kShr8>(0.0f, v);
+  v += dpp<kBcast15, 0xa>(0.0f, v);
+  v += dpp<kBcast31, 0xc>(0.0f, v);
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
+}
+__device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return a > b ? a : b; }
+__device__ __forceinline__ unsigned over_wave(unsigned v)
+{
+  v = larger(v, (unsigned)dpp<kShr1>(0, (int)v));
+  v = larger(v, (unsigned)dpp<kShr2>(0, (int)v));
+  v = larger(v, (unsigned)dpp<kShr4>(0, (int)v));
+  v = larger(v, (unsigned)dpp<kShr8>(0, (int)v));
+  v = larger(v, (unsigned)dpp<kBcast15, 0xa>(0, (int)v));
+  v = larger(v, (unsigned)dpp<kBcast31, 0xc>(0, (int)v));
+  return (unsigned)__builtin_amdgcn_readlane((int)v, 63);
+}
 // Sum (or, of bit patterns without a sign, the maximum: a NaN's is above every number's, so it is kept) over the THREADS of a
 // row, the same bits in each of them
 template <int THREADS, typename T, typename Op>
 __device__ __forceinline__ T over_row(T v, T *room, Op op)
 {
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) v = op(v, __shfl_xor(v, d));
+  v = over_wave(v);
   if constexpr (THREADS > 64) {
     __syncthreads();   // the room's last readers
     if ((threadIdx.x & 63) == 0) room[threadIdx.x >> 6] = v;
@@ -74,12 +96,12 @@ __device__ __forceinline__ T over_row(T v, T *room, Op op)
   return v;
 }
 
-// THREADS threads have a row, each of them V runs of 8 columns, THREADS * 8 apart.  Two passes over the registers for the
+// THREADS threads have a row (64: four rows to a workgroup), each of them V runs of 8 columns, THREADS * 8 apart.  Two passes over the registers for the
 // variance of a layer norm: a row whose mean is large against its spread loses nothing.
 template <int TYPE, bool S8, int THREADS, int V>
-__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_norm(NormArgs a)
+__global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void k_norm(NormArgs a)
 {
-  constexpr int ROWS = THREADS < 256 ? 256 / THREADS : 1, SIZE = Elem<TYPE>::size;
+  constexpr int ROWS = THREADS == 64 ? 4 : 1, SIZE = Elem<TYPE>::size;
   __shared__ float froom[THREADS > 64 ? THREADS / 64 : 1];
   __shared__ unsigned uroom[THREADS > 64 ? THREADS / 64 : 1];
   const long long r = (long long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
@@ -187,7 +209,7 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_norm(NormArgs
         if (j < n && m > most) most = m;
       }
     }
-    most = over_row<THREADS>(most, uroom, [](unsigned x, unsigned y) { return x > y ? x : y; });
+    most = over_row<THREADS>(most, uroom, larger);
     const float amax = __builtin_bit_cast(float, most);
     // a row of zeros has codes 0 and scale 0; one with an infinity or a NaN says so in its scale
     const float lift = amax < 1e-30f ? 0x1p64f : 1.0f;   // 127 / amax stays finite
@@ -225,22 +247,25 @@ __global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void k_norm(NormArgs
 template <int TYPE, bool S8, int THREADS, int V>
 hipError_t run(const NormArgs &a, hipStream_t s)
 {
-  constexpr int rows = THREADS < 256 ? 256 / THREADS : 1;
+  constexpr int rows = THREADS == 64 ? 4 : 1;
   const long long blocks = (a.rows + rows - 1) / rows;
   if (blocks >= 1ll << 31) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_norm<TYPE, S8, THREADS, V>), dim3((unsigned)blocks), dim3(THREADS < 256 ? 256 : THREADS), 0, s, a);
+  hipLaunchKernelGGL((k_norm<TYPE, S8, THREADS, V>), dim3((unsigned)blocks), dim3(THREADS == 64 ? 256 : THREADS), 0, s, a);
   return hipGetLastError();
 }
 
+// Eight columns a thread as long as a workgroup has the threads, whatever the rows: bf16, us, against four times as many columns
+// a thread: 64 x 4096 3.7 (64 threads: 12.9), 16384 x 4096 113 (120 with 128, 181 with 64), 16384 x 1024 30 (64 threads: 39).
+// Above 8192 columns fewer waves that each have more in flight: 4096 x 16384 134, with 1024 threads 162.
 template <int TYPE, bool S8>
 hipError_t run_wide(const NormArgs &a, hipStream_t s)
 {
   if (a.cols <= 512) return run<TYPE, S8, 64, 1>(a, s);
-  if (a.cols <= 1024) return run<TYPE, S8, 64, 2>(a, s);
+  if (a.cols <= 1024) return run<TYPE, S8, 128, 1>(a, s);
   if (a.cols <= 2048) return run<TYPE, S8, 256, 1>(a, s);
   if (a.cols <= 4096) return run<TYPE, S8, 512, 1>(a, s);
   if (a.cols <= 8192) return run<TYPE, S8, 1024, 1>(a, s);
-  if (a.cols <= 16384) return run<TYPE, S8, 1024, 2>(a, s);
+  if (a.cols <= 16384) return run<TYPE, S8, 512, 4>(a, s);
   if (a.cols <= 32768) return run<TYPE, S8, 1024, 4>(a, s);
   return run<TYPE, S8, 1024, 8>(a, s);
 }

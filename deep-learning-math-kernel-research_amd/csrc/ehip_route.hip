@@ -16,19 +16,6 @@ namespace {
 
 constexpr float kClosed = -__builtin_inff();
 
-// v of the lane that DPP control CTRL names; lanes without one, or outside of ROWS, keep `old`
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ int dpp(int old, int v)
-{
-  return __builtin_amdgcn_update_dpp(old, v, CTRL, ROWS, 0xf, false);
-}
-template <int CTRL, int ROWS = 0xf>
-__device__ __forceinline__ float dpp(float old, float v)
-{
-  return __builtin_bit_cast(float, dpp<CTRL, ROWS>(__builtin_bit_cast(int, old), __builtin_bit_cast(int, v)));
-}
-constexpr int kShr1 = 0x111, kShr2 = 0x112, kShr4 = 0x114, kShr8 = 0x118, kBcast15 = 0x142, kBcast31 = 0x143;
-
 // Keys are compared as integers of the same order (a zero has no sign): one instruction each, where a maximum of floats takes
 // three to keep a signalling NaN quiet.
 __device__ __forceinline__ int ordered(float v)
