@@ -171,14 +171,31 @@ struct Field {
   size_t offset;
 };
 
+// The names of keyword arguments are interned where they stand in a caller's source: mostly one comparison of pointers each
 template <int N>
-PyObject *layer_execute(PyObject *self, const char *fn, layer_t f, const Field (&fields)[N], int required, PyObject *const *args, Py_ssize_t nargs,
-                        PyObject *kwnames, char *block)
+PyObject *layer_execute(PyObject *self, const char *fn, layer_t f, const Field (&fields)[N], PyObject *(&interned)[N], int required,
+                        PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames, char *block)
 {
-  const char *names[N];
-  for (int i = 0; i < N; ++i) names[i] = fields[i].name;
   PyObject *v[N];
-  if (!arguments(fn, names, required, args, nargs, kwnames, v)) return nullptr;
+  const Py_ssize_t nkw = kwnames ? PyTuple_GET_SIZE(kwnames) : 0;
+  bool plain = nargs <= N;
+  if (plain) {
+    for (int i = 0; i < N; ++i) v[i] = i < nargs ? args[i] : nullptr;
+    int i = 0;   // (keywords mostly come in the order of the fields)
+    for (Py_ssize_t k = 0; k < nkw && plain; ++k) {
+      PyObject *name = PyTuple_GET_ITEM(kwnames, k);
+      int looked = 0;
+      for (; looked < N && interned[i] != name; ++looked) i = i + 1 < N ? i + 1 : 0;
+      plain = looked < N && !v[i];
+      if (plain) v[i] = args[nargs + k];
+    }
+    for (int r = 0; r < required; ++r) plain = plain && v[r];
+  }
+  if (!plain) {   // a name that is not interned, or an argument list that is wrong
+    const char *names[N];
+    for (int i = 0; i < N; ++i) names[i] = fields[i].name;
+    if (!arguments(fn, names, required, args, nargs, kwnames, v)) return nullptr;
+  }
   void *stream = nullptr;
   for (int i = 0; i < N; ++i) {
     const Field &d = fields[i];
@@ -208,6 +225,14 @@ PyObject *layer_execute(PyObject *self, const char *fn, layer_t f, const Field (
   return result(rc);
 }
 
+template <int N>
+bool intern(const Field (&fields)[N], PyObject *(&interned)[N])
+{
+  for (int i = 0; i < N && !interned[N - 1]; ++i)
+    if (!interned[i] && !(interned[i] = PyUnicode_InternFromString(fields[i].name))) return false;
+  return true;
+}
+
 #define F(S, name, kind, field) {name, kind, offsetof(S, field)}
 PyObject *linear_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
 {
@@ -216,8 +241,10 @@ PyObject *linear_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs
                                  F(S, "input_scale", 'p', input_scale_dev), F(S, "residual", 'p', residual_dev),
                                  F(S, "output_stride", 'q', output_stride), F(S, "input_stride", 'q', input_stride),
                                  F(S, "residual_stride", 'q', residual_stride), {"stream", 's', 0}};
+  static PyObject *interned[sizeof(fields) / sizeof(fields[0])];
+  if (!intern(fields, interned)) return nullptr;
   S block = {};
-  return layer_execute(self, "execute", g_linear, fields, 3, args, nargs, kwnames, reinterpret_cast<char *>(&block));
+  return layer_execute(self, "execute", g_linear, fields, interned, 3, args, nargs, kwnames, reinterpret_cast<char *>(&block));
 }
 PyObject *experts_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
 {
@@ -227,8 +254,10 @@ PyObject *experts_execute(PyObject *self, PyObject *const *args, Py_ssize_t narg
                                  F(S, "input_scale", 'p', input_scale_dev), F(S, "input_rows", 'i', input_rows),
                                  F(S, "output_rows", 'i', output_rows), F(S, "output_stride", 'q', output_stride),
                                  F(S, "input_stride", 'q', input_stride), {"stream", 's', 0}};
+  static PyObject *interned[sizeof(fields) / sizeof(fields[0])];
+  if (!intern(fields, interned)) return nullptr;
   S block = {};
-  return layer_execute(self, "execute_experts", g_experts, fields, 6, args, nargs, kwnames, reinterpret_cast<char *>(&block));
+  return layer_execute(self, "execute_experts", g_experts, fields, interned, 6, args, nargs, kwnames, reinterpret_cast<char *>(&block));
 }
 PyObject *norm_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
 {
@@ -241,8 +270,10 @@ PyObject *norm_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, 
                                  F(S, "output_stride", 'q', output_stride), F(S, "sum_stride", 'q', sum_stride),
                                  F(S, "block_stride", 'q', block_stride), F(S, "residual_stride", 'q', residual_stride),
                                  F(S, "gate_stride", 'q', gate_stride), {"stream", 's', 0}};
+  static PyObject *interned[sizeof(fields) / sizeof(fields[0])];
+  if (!intern(fields, interned)) return nullptr;
   S block = {};
-  return layer_execute(self, "execute", g_norm, fields, 3, args, nargs, kwnames, reinterpret_cast<char *>(&block));
+  return layer_execute(self, "execute", g_norm, fields, interned, 3, args, nargs, kwnames, reinterpret_cast<char *>(&block));
 }
 PyObject *route_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs, PyObject *kwnames)
 {
@@ -250,8 +281,10 @@ PyObject *route_execute(PyObject *self, PyObject *const *args, Py_ssize_t nargs,
   static const Field fields[] = {F(S, "ids", 'p', ids_dev), F(S, "weights", 'p', weights_dev), F(S, "plan", 'p', plan_dev),
                                  F(S, "logits", 'p', logits_dev), F(S, "tokens", 'q', tokens), F(S, "bias", 'p', bias_dev),
                                  F(S, "logits_stride", 'q', logits_stride), {"stream", 's', 0}};
+  static PyObject *interned[sizeof(fields) / sizeof(fields[0])];
+  if (!intern(fields, interned)) return nullptr;
   S block = {};
-  return layer_execute(self, "execute", g_route, fields, 5, args, nargs, kwnames, reinterpret_cast<char *>(&block));
+  return layer_execute(self, "execute", g_route, fields, interned, 5, args, nargs, kwnames, reinterpret_cast<char *>(&block));
 }
 #undef F
 
