@@ -67,6 +67,9 @@ hipError_t launch_linear_constants(float *dst, const float *src, int experts, in
 // come by whole lines, 8 lanes a row, and change lanes through a corner of LDS that is the wave's own (a load that gave every
 // lane the 16 bytes that its matrix operand has would be 64 accesses instead of 16, and the loads bound these kernels).  The
 // waves' sums meet in LDS, in the order of the waves.
+// Measured: bf16 1 x 4096 x 4096 7.2 us, 4.6 TB/s of weights; s8 gated 16 x 4096 x 8192 12.2 us, 5.5 TB/s; f16 64 x 2048 x 1000
+// 3.9 us; 64 slots of 32 experts of 2048 x 2816 57 us, 5.7 TB/s.  Weights' bytes bound it up to some 16 rows, then the loads:
+// 64 x 64 results of 64 steps take a CU 11 us, twice what their products do.
 template <int TYPE, int NT, int MT, int P>
 __global__ __launch_bounds__(512) void k_linear_split(LinearArgs a)
 {

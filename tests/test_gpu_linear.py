@@ -93,6 +93,25 @@ def test_epilogues(m, ic, oc, gated, activation):
         c.check()
 
 
+@pytest.mark.parametrize("form", range(9))
+@pytest.mark.parametrize("itype", TYPES)
+@pytest.mark.parametrize("m, ic, oc, gap", [(7, 520, 70, 0), (70, 704, 150, 8), (140, 333, 77, 3), (290, 1280, 260, 0)])
+def test_every_form(m, ic, oc, gap, itype, form, monkeypatch):
+    """the kernel forms at sizes that the choice would not give them; rows at multiples of 16 bytes and others"""
+    monkeypatch.setenv("EHIP_LINEAR_FORM", str(form))
+    for gated in (False, True):
+        c = Case(m, ic, oc, itype, E.BF16 if gated else E.F32, activation=E.ACT_GELU, gated=gated, bias=True, residual=True, gap=gap)
+        c.run()
+        c.check()
+
+
+@pytest.mark.parametrize("form", range(9))
+def test_experts_in_every_form(form, monkeypatch):
+    monkeypatch.setenv("EHIP_LINEAR_FORM", str(form))
+    test_experts(400, 5, 2, 264, 130, E.BF16, "up")
+    test_experts(60, 9, 3, 96, 48, E.S8, "down")
+
+
 @pytest.mark.parametrize("m", [1, 40, 300])
 def test_residual_in_place(m):
     c = Case(m, 192, 100, E.BF16, E.BF16, residual=True, gap=4)
