@@ -183,12 +183,28 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
         *reinterpret_cast<Acc *>(to + t / 4 * 256 + (GATED ? t % 2 * 128 + t % 4 / 2 * 16 : t % 4 * 16)) = acc[n][mc.value];
       }
     };
+    constexpr int RUNS = WM * 16 / HIGH;   // rows of a thread in a pass
+    auto row_at = [&](int k, int m) {
+      const long long p = blk.first + ((row0 / 16 + k * (HIGH / 16)) * MTW + m) * 16 + row0 % 16;
+      return live && p < blk.last ? row_of(a, p) : RowOf{0, 0, false};
+    };
+    // whole runs of the residual are on their way while the results before them cross LDS
+    typedef unsigned Old __attribute__((ext_vector_type(2 * SIZE), aligned(2)));
+    Old old[RUNS];
+    const bool early = a.res && a.oc - col >= 8;
+    auto fetch_old = [&](int m) {
+      if (!early) return;
+#pragma unroll
+      for (int k = 0; k < RUNS; ++k) {
+        const RowOf row = row_at(k, m);
+        if (row.there) old[k] = *reinterpret_cast<const Old *>(a.res + row.out * a.ldr + (long long)col * SIZE);
+      }
+    };
     auto read = [&](int m) {
 #pragma unroll
-      for (int k = 0; k < WM * 16 / HIGH; ++k) {
-        const long long p = blk.first + ((row0 / 16 + k * (HIGH / 16)) * MTW + m) * 16 + row0 % 16;
-        const RowOf row = p < blk.last ? row_of(a, p) : RowOf{0, 0, false};
-        if (!live || !row.there) continue;
+      for (int k = 0; k < RUNS; ++k) {
+        const RowOf row = row_at(k, m);
+        if (!row.there) continue;
         const float xs = a.xscale ? a.xscale[row.in] : 1.0f;
         float v[1 + GATED][8];
 #pragma unroll
@@ -207,8 +223,23 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
           v[0][j] = activate<act.value>(v[0][j]);
           if (GATED) v[0][j] *= v[GATED][j];
         }
+        if (early) {
+#pragma unroll
+          for (int j = 0; j < 8; j += 2) {
+            float lo, hi;
+            if (SIZE == 4) {
+              const unsigned a0 = old[k][j], a1 = old[k][j + 1];
+              lo = __builtin_bit_cast(float, a0);
+              hi = __builtin_bit_cast(float, a1);
+            } else {
+              unpack(old[k][j / 2], type.value == EHIP_BF16, lo, hi);
+            }
+            v[0][j] = __builtin_fmaf(a.res_scale, lo, v[0][j]);
+            v[0][j + 1] = __builtin_fmaf(a.res_scale, hi, v[0][j + 1]);
+          }
+        }
         store_columns<type.value, 8>(v[0], a.out + row.out * a.ldo + (long long)col * SIZE,
-                                     a.res ? a.res + row.out * a.ldr + (long long)col * SIZE : nullptr, a.res_scale, a.oc - col);
+                                     a.res && !early ? a.res + row.out * a.ldr + (long long)col * SIZE : nullptr, a.res_scale, a.oc - col);
       }
     };
     auto pass = [&](auto mc) {
@@ -216,8 +247,10 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
       write(mc);
       __syncthreads();
       read(mc.value);
+      if (mc.value + 1 < MTW) fetch_old(mc.value + 1);
     };
     static_assert(MTW == 4, "four passes");
+    fetch_old(0);
     pass(Const<0>());
     pass(Const<1>());
     pass(Const<2>());
