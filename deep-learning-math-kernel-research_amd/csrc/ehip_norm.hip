@@ -111,7 +111,7 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void k_norm(NormArgs
   const float inv = 1.0f / (float)a.cols;
 
   float v[V][8];
-  if (a.parts == 1) {
+  if (a.parts == 1 && !a.pw) {
 #pragma unroll
     for (int i = 0; i < V; ++i) {
       const int col = (i * THREADS + t) * 8;

@@ -260,7 +260,7 @@ EHIP_API int ehip_linear_execute_experts(const ehip_linear_t *linear, const ehip
 EHIP_API const char *ehip_linear_kernel_name(const ehip_linear_t *linear, int64_t rows);
 
 /* The norm after a block, its gate and residual scale, and the norm before the next block, in one pass over the rows:
- *   y = block[r]   (parts > 1: sum over j of part_weights[r][j] * block[r * parts + j]; a part of weight 0 is not read)
+ *   y = block[r]   (with part_weights: sum over j of part_weights[r][j] * block[r * parts + j]; a part of weight 0 is not read)
  *   h = residual_scale * residual[r] + block_scale * gate[r / rows_per_gate] * post(y)
  *   sum[r] = h,  output[r] = pre(h)
  * RMS: x / sqrt(mean(x^2) + eps) * weight + bias, LAYER: the same of x - mean(x).  Weights and biases f32, null = 1 and 0.
@@ -279,7 +279,7 @@ typedef struct ehip_norm_args {
   float *output_scale_dev;           /* s8 output                                                              */
   void *sum_dev;                     /* null: not wanted; may be the residual itself (same stride)             */
   const void *block_dev, *residual_dev /* or null */, *gate_dev /* or null */;
-  const float *part_weights_dev;     /* [rows][parts], with parts > 1                                          */
+  const float *part_weights_dev;     /* [rows][parts]; null with parts = 1: a weight of 1                      */
   const float *post_weight_dev, *post_bias_dev, *pre_weight_dev, *pre_bias_dev;
   int64_t rows;
   int64_t output_stride, sum_stride, block_stride, residual_stride, gate_stride;

@@ -1,5 +1,6 @@
 """A routed feed-forward block end to end: linear, norm, route and experts in the order a model runs them, against 64 bits."""
 import importlib
+import math
 
 import pytest
 import torch
@@ -64,3 +65,50 @@ def test_block(tokens, width, hidden, experts, topk, dtype):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(x2, out)
+
+
+@pytest.mark.parametrize("dtype", [E.BF16, E.F16])
+@pytest.mark.parametrize("tokens", [1, 70, 300])
+@pytest.mark.parametrize("topk, scale", [(1, 2.5), (1, 1.0), (2, 2.5)])
+def test_one_choice_and_tokens_without_an_expert(tokens, topk, scale, dtype):
+    """the routing weight counts with one choice, too; a token whose experts are all closed keeps its residual"""
+    block = ff.RoutedFeedForward(128, 64, 8, topk, data_type=dtype, scale=scale)
+    w = ff.synthetic(block, seed=tokens)
+    g = torch.Generator(device="cuda")
+    g.manual_seed(tokens)
+    x = torch.randn((tokens, 128), generator=g, device="cuda").to(block.dtype)
+    if tokens > 1:
+        x[1] = math.nan   # its logits are NaN: every expert is closed to it
+    out, normed, b = torch.empty_like(x), torch.empty_like(x), block.buffers(tokens)
+    for t in (b["hidden"], b["y"]):
+        t.fill_(math.nan)   # what no position writes
+    block.execute(out, normed, x, tokens, b)
+    torch.cuda.synchronize()
+    live = [t for t in range(tokens) if t != 1]
+    assert (b["ids"][live] >= 0).all()
+    if topk == 1:
+        assert torch.equal(b["weights"][live], torch.full((len(live), 1), scale, device="cuda"))
+    _, h, n = reference(block, w, x[live], b["ids"][live], b["weights"][live])
+    u = ref.ROUND[block.dtype][0]
+    for got, want in ((out[live], h), (normed[live], n)):
+        off = torch.linalg.norm(got.double() - want) / torch.linalg.norm(want)
+        assert off <= 2 * 4 * u, float(off)   # (four roundings, as above)
+    if tokens > 1:
+        assert (b["ids"][1] == -1).all() and (b["weights"][1] == 0).all() and torch.isnan(out[1]).all()
+
+
+@pytest.mark.parametrize("tokens", [6, 200])
+def test_a_closed_token_keeps_its_residual(tokens):
+    """the block's parts by themselves, with logits of -inf: what comes out is what came in"""
+    block = ff.RoutedFeedForward(128, 64, 8, 1, scale=2.5)
+    ff.synthetic(block)
+    x = torch.randn((tokens, 128), device="cuda").bfloat16()
+    out, normed, b = torch.empty_like(x), torch.empty_like(x), block.buffers(tokens)
+    b["y"].fill_(math.nan)
+    block.prepare(router=torch.zeros((8, 128), device="cuda").bfloat16(), up=torch.zeros((8, 128, 128), device="cuda").bfloat16(),
+                  down=torch.zeros((8, 128, 64), device="cuda").bfloat16(), norm_in=torch.ones(128, device="cuda"), norm_out=torch.ones(128, device="cuda"),
+                  bias=torch.full((8,), -math.inf, device="cuda"))
+    block.execute(out, normed, x, tokens, b)
+    torch.cuda.synchronize()
+    assert (b["ids"] == -1).all()
+    assert torch.equal(out, x) and torch.isfinite(normed).all()

@@ -127,6 +127,24 @@ def test_parts_of_weight_zero_are_not_read():
     c.check()
 
 
+@pytest.mark.parametrize("cols", [200, 900, 3000])
+@pytest.mark.parametrize("dtype", [E.BF16, E.F32])
+def test_a_single_part_has_its_weight(cols, dtype):
+    c = Case(9, cols, dtype, post=E.NORM_NONE, gap=3)
+    w = torch.rand((9, 1), device="cuda") + 1.5
+    w[4] = 0   # a row that nothing wrote: not read
+    c.y[4] = math.nan
+    c.run(part_weights=w)
+    torch.cuda.synchronize()
+    # the product that the weight makes, off by one rounding, in the block's place
+    c.y[4] = 0
+    p = w.double() * c.y.double()
+    (h, eh), (o, eo) = ref.norm(c.d, 9, p, c.r, None, None, c.w1, c.b1, c.w2, c.b2)
+    off = 2 * ref.EPS32 * c.d.block_scale * p.abs()
+    ref.close(c.sum, h, eh + off)
+    ref.close(c.out, *ref.one_norm(h, eh + off, c.d.pre, c.d.pre_eps, c.w2, c.b2))
+
+
 def test_rows_of_zeros_and_of_what_is_no_number():
     c = Case(5, 300, E.F32, out=E.S8, pre=E.NORM_NONE, residual=False)
     c.y[0] = 0
