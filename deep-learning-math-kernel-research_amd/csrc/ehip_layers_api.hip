@@ -92,6 +92,9 @@ int linear_args(const ehip_linear *h, const ehip_linear_args_t &g, LinearArgs *a
   if (!stride(g.input_stride, d.ic, h->elem, &a->ldx) || !stride(g.output_stride, d.oc, osize, &a->ldo) ||
       !stride(g.residual_stride, d.oc, osize, &a->ldr))
     return fail(EHIP_GENERAL_ERROR, "linear: a stride is shorter than a row or out of range");
+  // what the descriptor has no place for would be left out without a word
+  if (g.residual_dev && !d.with_residual) return fail(EHIP_GENERAL_ERROR, "linear: a residual, but not with_residual");
+  if (g.input_scale_dev && d.input_type != EHIP_S8) return fail(EHIP_GENERAL_ERROR, "linear: input scales are for s8 rows");
   if (g.rows > 0) {
     if (!g.output_dev || !g.input_dev || (d.input_type == EHIP_S8 && !g.input_scale_dev) || (d.with_residual && !g.residual_dev))
       return fail(EHIP_GENERAL_ERROR, "linear: null argument");
@@ -173,6 +176,8 @@ EHIP_API int ehip_linear_prepare(ehip_linear_t *h, const void *weights_dev, cons
     const ehip_linear_desc_t &d = h->d;
     if (d.input_type == EHIP_S8 && !scale_dev) return fail(EHIP_GENERAL_ERROR, "linear: s8 weights come with a scale per row");
     if (d.with_bias && !bias_dev) return fail(EHIP_GENERAL_ERROR, "linear: with_bias, but no bias");
+    if (d.input_type != EHIP_S8 && scale_dev) return fail(EHIP_GENERAL_ERROR, "linear: scales are for s8 weights");
+    if (!d.with_bias && bias_dev) return fail(EHIP_GENERAL_ERROR, "linear: a bias, but not with_bias");
     if (!aligned(weights_dev, h->elem) || !aligned(scale_dev, 4) || !aligned(bias_dev, 4))
       return fail(EHIP_GENERAL_ERROR, "linear: an address is not a multiple of its elements' size");
     const hipStream_t s = static_cast<hipStream_t>(hip_stream);
@@ -189,6 +194,7 @@ EHIP_API int ehip_linear_execute(const ehip_linear_t *h, const ehip_linear_args_
   return guarded([&]() -> int {
     if (!h || !args) return fail(EHIP_GENERAL_ERROR, "null argument");
     if (h->d.experts != 1) return fail(EHIP_GENERAL_ERROR, "linear: a handle of experts is executed with their offsets");
+    if (args->slots_dev || args->offsets_dev) return fail(EHIP_GENERAL_ERROR, "linear: slots and offsets are for ehip_linear_execute_experts");
     LinearArgs a;
     const int rc = linear_args(h, *args, &a);
     if (rc != EHIP_OK || args->rows == 0) return rc;
@@ -280,6 +286,7 @@ EHIP_API int ehip_norm_execute(const ehip_norm_t *h, const ehip_norm_args_t *arg
         !stride(g.block_stride, d.cols, size, &a.ldb) || !stride(g.residual_stride, d.cols, size, &a.ldr) ||
         !stride(g.gate_stride, d.cols, size, &a.ldg))
       return fail(EHIP_GENERAL_ERROR, "norm: a stride is shorter than a row or out of range");
+    if (g.output_scale_dev && d.output_type != EHIP_S8) return fail(EHIP_GENERAL_ERROR, "norm: output scales are for s8 rows");
     if (g.rows == 0) return EHIP_OK;
     if (!g.block_dev || (!g.output_dev && !g.sum_dev) || (d.parts > 1 && !g.part_weights_dev) ||
         (d.output_type == EHIP_S8 && g.output_dev && !g.output_scale_dev))

@@ -208,7 +208,8 @@ EHIP_API int ehip_reorder_oihw_to_blocked(void *dst_dev, const void *src_dev, in
 /* ---- the layers between convolutions: linear, norm, route, experts --------------------------------------------------
  * No counterpart in the reference.  Activations are rows of features, row-major; a stride is the distance of two rows
  * in elements, 0 meaning rows without a gap.  Addresses need the alignment of their elements only.  No rows is a call
- * that does nothing.  Handles hold constants (packed weights) and nothing of a call: executes of one handle may overlap
+ * that does nothing.  A tensor that the descriptor has no use for (a residual without with_residual, a bias without
+ * with_bias, scales without s8) is refused; the weight and bias of a norm that is EHIP_NORM_NONE are not read.  Handles hold constants (packed weights) and nothing of a call: executes of one handle may overlap
  * on several streams, and every call can be captured into a graph. */
 
 /* activation functions: erf form of GELU; silu(x) = x / (1 + exp(-x)) */

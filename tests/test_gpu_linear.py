@@ -1,6 +1,7 @@
 """Linear and the experts' products on the GPU against 64 bits: every kernel, type and epilogue at the sizes where a tile, a
 chunk of K or a vector ends, rows with gaps, any alignment.  What lies around the tensors is NaN or a mark, so that a read or a
 write past an edge shows."""
+import ctypes
 import math
 
 import pytest
@@ -261,4 +262,36 @@ def test_calls_are_checked_before_a_launch():
                             ((256, 256, 256, 256, 1 << 30, 2), {}, "2\\^30"), ((256, 256, 258, 256, 4, 2), {}, "multiple")):
         with pytest.raises(E.EulerHipError, match=match):
             h.execute_experts(*args, **kw)
+    torch.cuda.synchronize()
+
+
+def test_tensors_without_a_use_are_refused():
+    """not left out without a word"""
+    w, v = torch.zeros((32, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros(32, device="cuda")
+    x, out = torch.zeros((4, 64), dtype=torch.bfloat16, device="cuda"), torch.zeros((4, 32), dtype=torch.bfloat16, device="cuda")
+    plain = E.Linear(E.make_linear_desc(64, 32))
+    for kw, match in (({"bias": v}, "not with_bias"), ({"scale": v}, "s8 weights")):
+        with pytest.raises(E.EulerHipError, match=match):
+            plain.prepare(w, **kw)
+    plain.prepare(w)
+    for kw, match in (({"residual": out}, "not with_residual"), ({"input_scale": v}, "s8 rows")):
+        with pytest.raises(E.EulerHipError, match=match):
+            plain.execute(out, x, 4, **kw)
+    experts = E.Linear(E.make_linear_desc(64, 32, experts=2))
+    experts.prepare(torch.zeros((2, 32, 64), dtype=torch.bfloat16, device="cuda"))
+    slots, offsets = torch.arange(4, dtype=torch.int32, device="cuda"), torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    with pytest.raises(E.EulerHipError, match="s8 rows"):
+        experts.execute_experts(out, x, slots, offsets, 4, 2, input_scale=v)
+
+    class Args(ctypes.Structure):   # ehip_linear_args_t: what the Python call has no names for
+        _fields_ = [(k, ctypes.c_void_p) for k in ("output", "input", "input_scale", "residual", "slots", "offsets")] + [
+            (k, ctypes.c_int64) for k in ("rows", "output_stride", "input_stride", "residual_stride")] + [
+            (k, ctypes.c_int32) for k in ("topk", "input_rows", "output_rows")]
+
+    for kw in ({"slots": slots.data_ptr()}, {"offsets": offsets.data_ptr()}):
+        args = Args(output=out.data_ptr(), input=x.data_ptr(), rows=4, **kw)
+        assert E.lib.ehip_linear_execute(plain._h, ctypes.byref(args), None) == E.EHIP_GENERAL_ERROR
+    args = Args(output=out.data_ptr(), input=x.data_ptr(), rows=4, residual=out.data_ptr(), slots=slots.data_ptr(), offsets=offsets.data_ptr(), topk=2)
+    assert E.lib.ehip_linear_execute_experts(experts._h, ctypes.byref(args), None) == E.EHIP_GENERAL_ERROR
+    plain.execute(out, x, 4)
     torch.cuda.synchronize()

@@ -92,3 +92,11 @@ def test_argument_lists(base):
             h.execute(256, 256, np.int64(4))
         with pytest.raises(OverflowError):
             h.execute(256, 256, 1 << 70)
+
+
+@pytest.mark.parametrize("kind", [E.F32, E.F16, E.BF16])
+def test_scales_without_codes_are_refused(kind):
+    h = E.Norm(E.make_norm_desc(64, data_type=kind))
+    for rows in (0, 4):
+        with pytest.raises(E.EulerHipError, match="s8 rows"):
+            h.execute(256, 256, rows, output_scale=256)
