@@ -15,6 +15,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libeuler_hip.so")
 
 SOURCES = [
+    "ehip_linear_tile_bf16.hip", "ehip_linear_tile_f16.hip", "ehip_linear_tile_s8.hip",   # (the longest first)
+    "ehip_linear.hip",
     "ehip_gemm.hip",
     "ehip_gemm1x1.hip",
     "ehip_gemm1x1w.hip",
@@ -30,7 +32,6 @@ SOURCES = [
     "ehip_wino_whole.hip", "ehip_wino_whole6.hip", "ehip_wino_whole5.hip", "ehip_wino_whole4.hip",
     "ehip_prepare.hip",
     "ehip_harness.hip",
-    "ehip_linear.hip", "ehip_linear_tile.hip",
     "ehip_norm.hip",
     "ehip_route.hip",
     "ehip_layers_api.hip",
@@ -73,7 +74,8 @@ EXTRA_FLAGS = {
     "ehip_gemm1x1w.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16", "-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     # the 128 x 128 form's accumulators: in the accumulation registers half of them would be moved around each product.  m0, which
     # the loads into LDS set, is a register that the compiler keeps to itself
-    "ehip_linear_tile.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-pragma-unroll-threshold=1000000", "-Wno-inline-asm"],
+    **{"ehip_linear_tile_%s.hip" % t: ["-mllvm", "-amdgpu-mfma-vgpr-form=1", "-mllvm", "-pragma-unroll-threshold=1000000", "-Wno-inline-asm"]
+       for t in ("bf16", "f16", "s8")},
     "ehip_linear.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
     # and those of the 1x1 kernels with few input channels
     "ehip_gemm.hip": ["-mllvm", "-amdgpu-kernarg-preload-count=16"],

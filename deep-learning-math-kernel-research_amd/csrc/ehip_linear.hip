@@ -1,8 +1,7 @@
 // Products of rows of activations with a matrix (or with the matrices of the experts they are sent to), few rows: the K
 // axis shared out among the waves of a workgroup, operands straight from memory to registers.  Also the packing of the
-// weights, and the choice between this kernel and the one that stages tiles in LDS (ehip_linear_tile.hip).
+// weights, and the choice between this kernel and the one that stages tiles in LDS (ehip_linear_tile.hpp).
 #include "ehip_layers.hpp"
-#include "ehip_linear_tile.hpp"
 
 namespace ehip {
 
@@ -295,6 +294,7 @@ Form choose(const LinearArgs &a)
 template <int TYPE>
 hipError_t launch_typed(const LinearArgs &a, hipStream_t s)
 {
+  auto tile = TYPE == EHIP_BF16 ? launch_linear_tile_bf16 : TYPE == EHIP_F16 ? launch_linear_tile_f16 : launch_linear_tile_s8;
   switch (choose(a)) {
   case SPLIT_1X1: return run_split<TYPE, 1, 1, 4>(a, s);
   case SPLIT_2X1: return run_split<TYPE, 2, 1, 4>(a, s);
@@ -302,9 +302,9 @@ hipError_t launch_typed(const LinearArgs &a, hipStream_t s)
   case SPLIT_2X2: return run_split<TYPE, 2, 2, 3>(a, s);
   case SPLIT_4X2: return run_split<TYPE, 4, 2, 2>(a, s);
   case SPLIT_4X4: return run_split<TYPE, 4, 4, 2>(a, s);
-  case TILE_128: return launch_linear_tile(a, TYPE, 0, blocks_of(a, 128), s);
-  case TILE_128_DEEP: return launch_linear_tile(a, TYPE, 1, blocks_of(a, 128), s);
-  default: return launch_linear_tile(a, TYPE, 2, blocks_of(a, 256), s);
+  case TILE_128: return tile(a, 0, blocks_of(a, 128), s);
+  case TILE_128_DEEP: return tile(a, 1, blocks_of(a, 128), s);
+  default: return tile(a, 2, blocks_of(a, 256), s);
   }
 }
 
