@@ -45,7 +45,7 @@ hipError_t launch_linear_pack(void *packed, const void *weights, int experts, in
                               char *zeros, hipStream_t s);
 hipError_t launch_linear_constants(float *dst, const float *src, int experts, int oc, int gated, int tiles, hipStream_t s);
 hipError_t launch_linear(const LinearArgs &a, int type, hipStream_t s);
-const char *linear_kernel_name(const LinearArgs &a, int type);
+const char *linear_kernel_name(const LinearArgs &a);   // for rows without gaps, at multiples of 16 bytes
 // many rows: tiles of 128 x 128 (form 0; form 1: four steps in LDS) or 256 x 256 (form 2) results staged through LDS
 hipError_t launch_linear_tile_bf16(const LinearArgs &a, int form, long long blocks_m, hipStream_t s);
 hipError_t launch_linear_tile_f16(const LinearArgs &a, int form, long long blocks_m, hipStream_t s);

@@ -81,13 +81,35 @@ int linear_check(const ehip_linear_desc_t &d)
   return EHIP_OK;
 }
 
+// what the handle has for every call
+LinearArgs constant_args(const ehip_linear *h)
+{
+  const ehip_linear_desc_t &d = h->d;
+  LinearArgs a = {};
+  a.w = h->packed;
+  a.wscale = d.input_type == EHIP_S8 ? h->scale : nullptr;
+  a.bias = d.with_bias ? h->bias : nullptr;
+  a.zeros = h->zeros;
+  a.oc = d.oc;
+  a.kbytes = d.ic * h->elem;
+  a.tiles = h->tiles;
+  a.chunks = h->chunks;
+  a.experts = d.experts;
+  a.out_type = d.output_type;
+  a.act = d.activation;
+  a.gated = d.gated;
+  a.res_scale = d.residual_scale;
+  a.form = h->form;
+  return a;
+}
+
 // what both executes check; fills the kernel's arguments
 int linear_args(const ehip_linear *h, const ehip_linear_args_t &g, LinearArgs *a)
 {
   const ehip_linear_desc_t &d = h->d;
   if (!h->prepared) return fail(EHIP_GENERAL_ERROR, "linear: not prepared");
   if (g.rows < 0 || g.rows >= kMaxRows) return fail(EHIP_GENERAL_ERROR, "linear: rows out of range");
-  *a = LinearArgs{};
+  *a = constant_args(h);
   const int osize = size_of(d.output_type);
   if (!stride(g.input_stride, d.ic, h->elem, &a->ldx) || !stride(g.output_stride, d.oc, osize, &a->ldo) ||
       !stride(g.residual_stride, d.oc, osize, &a->ldr))
@@ -101,25 +123,11 @@ int linear_args(const ehip_linear *h, const ehip_linear_args_t &g, LinearArgs *a
     if (!aligned(g.output_dev, osize) || !aligned(g.input_dev, h->elem) || !aligned(g.residual_dev, osize) || !aligned(g.input_scale_dev, 4))
       return fail(EHIP_GENERAL_ERROR, "linear: an address is not a multiple of its elements' size");
   }
-  a->w = h->packed;
-  a->wscale = d.input_type == EHIP_S8 ? h->scale : nullptr;
-  a->bias = d.with_bias ? h->bias : nullptr;
-  a->zeros = h->zeros;
   a->x = static_cast<const char *>(g.input_dev);
   a->xscale = d.input_type == EHIP_S8 ? g.input_scale_dev : nullptr;
   a->out = static_cast<char *>(g.output_dev);
   a->res = d.with_residual ? static_cast<const char *>(g.residual_dev) : nullptr;
   a->rows = g.rows;
-  a->oc = d.oc;
-  a->kbytes = d.ic * h->elem;
-  a->tiles = h->tiles;
-  a->chunks = h->chunks;
-  a->experts = d.experts;
-  a->out_type = d.output_type;
-  a->act = d.activation;
-  a->gated = d.gated;
-  a->res_scale = d.residual_scale;
-  a->form = h->form;
   return EHIP_OK;
 }
 
@@ -232,18 +240,13 @@ EHIP_API int ehip_linear_execute_experts(const ehip_linear_t *h, const ehip_line
 EHIP_API const char *ehip_linear_kernel_name(const ehip_linear_t *h, int64_t rows)
 {
   if (!h || rows < 1 || rows >= kMaxRows) return "";
-  LinearArgs a = {};
+  LinearArgs a = constant_args(h);
   a.rows = rows;
-  a.oc = h->d.oc;
-  a.kbytes = h->d.ic * h->elem;
-  a.tiles = h->tiles;
-  a.chunks = h->chunks;
-  a.gated = h->d.gated;
-  a.experts = h->d.experts;
-  a.form = h->form;
+  // (of these only whether there are any is asked)
   static const int32_t none = 0;
-  if (h->d.experts > 1) a.offsets = &none;   // (only whether there are any is asked)
-  return linear_kernel_name(a, h->d.input_type);
+  if (h->d.experts > 1) a.offsets = &none;
+  if (h->d.with_residual) a.res = h->packed;
+  return linear_kernel_name(a);
 }
 
 EHIP_API int ehip_norm_create(const ehip_norm_desc_t *desc, ehip_norm_t **out)

@@ -319,12 +319,14 @@ hipError_t launch_linear(const LinearArgs &a, int type, hipStream_t s)
   }
 }
 
-const char *linear_kernel_name(const LinearArgs &a, int)
+const char *linear_kernel_name(const LinearArgs &a)
 {
   static const char *const names[FORMS] = {"k_linear_split<1x1>", "k_linear_split<2x1>", "k_linear_split<4x1>", "k_linear_split<2x2>",
                                            "k_linear_split<4x2>", "k_linear_split<4x4>", "k_linear_tile<128x128>",
                                            "k_linear_tile<128x128, deep>", "k_linear_tile<256x256>"};
-  return names[choose(a)];
+  const Form form = choose(a);
+  // rows that end at other bytes pass through registers, and there both 128 x 128 forms are one kernel
+  return names[form == TILE_128_DEEP && a.kbytes % 16 ? TILE_128 : form];
 }
 
 }  // namespace ehip

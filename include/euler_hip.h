@@ -257,7 +257,8 @@ EHIP_API int ehip_linear_execute(const ehip_linear_t *linear, const ehip_linear_
 /* The product of every position p in [offsets[e], offsets[e + 1]) with the matrix of expert e; no residual.  Output rows
  * that no position leads to are left as they are.  A slot outside [0, rows) is skipped. */
 EHIP_API int ehip_linear_execute_experts(const ehip_linear_t *linear, const ehip_linear_args_t *args, void *hip_stream);
-/* Name of the kernel that a call with so many rows runs. */
+/* Name of the kernel that ehip_linear_execute (experts > 1: ehip_linear_execute_experts) runs for so many rows without gaps, at
+ * addresses that are multiples of 16 bytes. */
 EHIP_API const char *ehip_linear_kernel_name(const ehip_linear_t *linear, int64_t rows);
 
 /* The norm after a block, its gate and residual scale, and the norm before the next block, in one pass over the rows:

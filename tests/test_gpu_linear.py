@@ -295,3 +295,32 @@ def test_tensors_without_a_use_are_refused():
     assert E.lib.ehip_linear_execute_experts(experts._h, ctypes.byref(args), None) == E.EHIP_GENERAL_ERROR
     plain.execute(out, x, 4)
     torch.cuda.synchronize()
+
+
+FORMS = ["k_linear_split<1x1>", "k_linear_split<2x1>", "k_linear_split<4x1>", "k_linear_split<2x2>", "k_linear_split<4x2>", "k_linear_split<4x4>",
+         "k_linear_tile<128x128>", "k_linear_tile<128x128, deep>", "k_linear_tile<256x256>"]
+
+
+@pytest.mark.parametrize("otype, residual, gated", [(E.F32, True, False), (E.BF16, False, False), (E.F32, True, True), (E.BF16, True, True)])
+@pytest.mark.parametrize("m, ic, oc", [(2048, 256, 512), (853, 704, 3392), (16, 1024, 512), (40, 512, 4096), (300, 1001, 640)])
+def test_the_name_is_of_the_kernel_that_runs(m, ic, oc, otype, residual, gated, monkeypatch):
+    """forms that share K out differently add in another order: the bits are those of the form that the name says"""
+    monkeypatch.delenv("EHIP_LINEAR_FORM", raising=False)
+    c = Case(m, ic, oc, E.BF16, otype, residual=residual, gated=gated)
+    c.run()
+    name = c.h.kernel_name(m)
+    monkeypatch.setenv("EHIP_LINEAR_FORM", str(FORMS.index(name)))
+    named = Case(m, ic, oc, E.BF16, otype, residual=residual, gated=gated)
+    named.run()
+    torch.cuda.synchronize()
+    assert named.h.kernel_name(m) == name
+    assert torch.equal(named.out, c.out), name
+    c.check()
+    if ic % 8:   # rows that end at other bytes than multiples of 16
+        assert name != "k_linear_tile<128x128, deep>"
+
+
+def test_the_name_counts_the_outputs_bytes():
+    """f32 results and their residual are four times the bytes of bf16 ones: another form is the faster one"""
+    names = [E.Linear(E.make_linear_desc(256, 512, output_type=t, with_residual=r)).kernel_name(2048) for t, r in ((E.BF16, False), (E.F32, True))]
+    assert names == ["k_linear_split<4x4>", "k_linear_tile<128x128, deep>"]
