@@ -39,6 +39,7 @@ struct LinearArgs {
   float res_scale;
   int form;                 // EHIP_LINEAR_FORM, or -1
   int blocks_m, blocks_n;   // set by the launcher
+  int first;                // number of the launch's first workgroup
 };
 
 hipError_t launch_linear_pack(void *packed, const void *weights, int experts, int oc, int ic, int elem, int gated, int tiles, int chunks,
@@ -61,6 +62,7 @@ struct NormArgs {
   long long rows;
   int cols, parts, post, pre, rows_per_gate;
   float block_scale, res_scale, eps1, eps2;
+  long long first;   // number of the launch's first workgroup
 };
 hipError_t launch_norm(const NormArgs &a, int type, int out_s8, hipStream_t s);
 
@@ -76,7 +78,21 @@ struct RouteArgs {
   float scale;
 };
 constexpr int kRouteBlock = 128;   // tokens of a workgroup
+constexpr long long kRouteTokens = (1ll << 29) - kRouteBlock;   // a launch's threads are counted in 32 bits, 8 a token
 hipError_t launch_route(const RouteArgs &a, int type, hipStream_t s);
+
+// A launch's threads are counted in 32 bits: more workgroups than that go out in pieces.  launch(number of the first, count)
+template <typename F>
+hipError_t launch_pieces(long long blocks, int threads, F launch)
+{
+  const long long most = ((1ll << 32) / threads - 1) / 8 * 8;   // (a workgroup's XCD stays its number modulo 8)
+  for (long long first = 0; first < blocks; first += most) {
+    launch(first, (unsigned)(blocks - first < most ? blocks - first : most));
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
 
 #if defined(__HIPCC__)
 

@@ -150,7 +150,7 @@ EHIP_API int ehip_linear_create(const ehip_linear_desc_t *desc, ehip_linear_t **
     h->tiles = desc->gated ? (desc->oc + 31) / 32 * 4 : (desc->oc + 63) / 64 * 4;
     h->chunks = (int)(((int64_t)desc->ic * h->elem + 127) / 128 * 2);
     const size_t blocks = (size_t)desc->experts * h->tiles * h->chunks, constants = (size_t)desc->experts * h->tiles * 16 * 4;
-    if (blocks * 64 >= (size_t)1 << 39) {   // the packing kernel's grid: 2^31 workgroups of 256
+    if (blocks >= (size_t)1 << 33) {   // 8 TiB: more than a card holds
       delete h;
       return fail(EHIP_UNIMPLEMENTED, "linear: the weights are too large");
     }
@@ -354,7 +354,7 @@ EHIP_API int ehip_route_destroy(ehip_route_t *h)
 
 EHIP_API int64_t ehip_route_plan_ints(const ehip_route_t *h, int64_t tokens)
 {
-  if (!h || tokens < 0 || tokens * h->d.topk >= 1ll << 30 || tokens >= 1ll << 30) return -1;
+  if (!h || tokens < 0 || tokens > kRouteTokens || tokens * h->d.topk >= 1ll << 30) return -1;
   const int64_t kept = tokens > kRouteBlock ? (1 + (tokens + kRouteBlock - 1) / kRouteBlock) * h->d.experts : 0;
   return h->d.experts + 1 + tokens * h->d.topk + kept;
 }

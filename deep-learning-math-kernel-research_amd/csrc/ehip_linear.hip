@@ -17,9 +17,9 @@ __device__ __forceinline__ int packed_source(int tile, int i, int oc, int gated,
 
 template <int ELEM>
 __global__ void k_linear_pack(char *packed, const char *w, int oc, int ic, int gated, int tiles, int chunks, long long units,
-                              char *zeros)
+                              char *zeros, long long first)
 {
-  const long long u = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const long long u = (first + blockIdx.x) * blockDim.x + threadIdx.x;
   if (u < 16) reinterpret_cast<i4 *>(zeros)[u] = i4{0, 0, 0, 0};
   if (u >= units) return;
   const int lane = (int)(u & 63);
@@ -48,9 +48,10 @@ hipError_t launch_linear_pack(void *packed, const void *weights, int experts, in
 {
   const long long units = (long long)experts * tiles * chunks * 64;
   auto kernel = elem == 1 ? k_linear_pack<1> : k_linear_pack<2>;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)((units + 255) / 256)), dim3(256), 0, s, static_cast<char *>(packed),
-                     static_cast<const char *>(weights), oc, ic, gated, tiles, chunks, units, zeros);
-  return hipGetLastError();
+  return launch_pieces((units + 255) / 256, 256, [&](long long first, unsigned count) {
+    hipLaunchKernelGGL(kernel, dim3(count), dim3(256), 0, s, static_cast<char *>(packed), static_cast<const char *>(weights), oc, ic, gated,
+                       tiles, chunks, units, zeros, first);
+  });
 }
 
 hipError_t launch_linear_constants(float *dst, const float *src, int experts, int oc, int gated, int tiles, hipStream_t s)
@@ -81,9 +82,9 @@ __global__ __launch_bounds__(512) void k_linear_split(LinearArgs a)
   const int g = lane >> 4, c = lane & 15;
 
   // blocks of the same weights beside each other on one XCD: its L2 holds them for all
-  const int per_xcd = (a.blocks_m * a.blocks_n + 7) / 8;
-  const int index = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per_xcd || index >= a.blocks_m * a.blocks_n) return;
+  const int per_xcd = (a.blocks_m * a.blocks_n + 7) / 8, number = a.first + (int)blockIdx.x;
+  const int index = (number & 7) * per_xcd + (number >> 3);
+  if (number >> 3 >= per_xcd || index >= a.blocks_m * a.blocks_n) return;
   const int bn = index / a.blocks_m;
   const Block blk = block_of(a, index - bn * a.blocks_m, 16 * MT);
   if (blk.expert < 0) return;
@@ -225,8 +226,10 @@ hipError_t run_split(LinearArgs a, hipStream_t s)
   if (all >= 1ll << 31) return hipErrorInvalidValue;
   a.blocks_m = (int)m;
   a.blocks_n = (int)n;
-  hipLaunchKernelGGL((k_linear_split<TYPE, NT, MT, P>), dim3((unsigned)all), dim3(512), 0, s, a);
-  return hipGetLastError();
+  return launch_pieces(all, 512, [&](long long first, unsigned count) {
+    a.first = (int)first;
+    hipLaunchKernelGGL((k_linear_split<TYPE, NT, MT, P>), dim3(count), dim3(512), 0, s, a);
+  });
 }
 
 enum Form { SPLIT_1X1, SPLIT_2X1, SPLIT_4X1, SPLIT_2X2, SPLIT_4X2, SPLIT_4X4, TILE_128, TILE_128_DEEP, TILE_256, FORMS };

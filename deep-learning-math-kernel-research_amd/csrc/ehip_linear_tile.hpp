@@ -32,9 +32,9 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
   const int g = lane >> 4, c = lane & 15;
 
   // blocks of an XCD are neighbours: 4 of rows x 8 of columns, so that 32 CUs share 12 panels in its L2
-  const int total = a.blocks_m * a.blocks_n, per_xcd = (total + 7) / 8;
-  const int index = (int)(blockIdx.x & 7) * per_xcd + (int)(blockIdx.x >> 3);
-  if ((int)(blockIdx.x >> 3) >= per_xcd || index >= total) return;
+  const int total = a.blocks_m * a.blocks_n, per_xcd = (total + 7) / 8, number = a.first + (int)blockIdx.x;
+  const int index = (number & 7) * per_xcd + (number >> 3);
+  if (number >> 3 >= per_xcd || index >= total) return;
   const int group = index / (4 * a.blocks_n), rest = index - group * 4 * a.blocks_n;
   const int high = a.blocks_m - group * 4 < 4 ? a.blocks_m - group * 4 : 4;
   const int bn = rest / high, bm = group * 4 + rest - bn * high;
@@ -273,8 +273,10 @@ hipError_t run(LinearArgs a, long long blocks_m, hipStream_t s)
   auto kernel = aligned ? k_linear_tile<TYPE, NTW, MTW, WN, WM, STAGES, true> : k_linear_tile<TYPE, NTW, MTW, WN, WM, 2, false>;
   const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, lds);
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)all), dim3(WN * WM * 64), lds, s, a);
-  return hipGetLastError();
+  return launch_pieces(all, WN * WM * 64, [&](long long first, unsigned count) {
+    a.first = (int)first;
+    hipLaunchKernelGGL(kernel, dim3(count), dim3(WN * WM * 64), lds, s, a);
+  });
 }
 
 }  // namespace

@@ -104,7 +104,7 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void k_norm(NormArgs
   constexpr int ROWS = THREADS == 64 ? 4 : 1, SIZE = Elem<TYPE>::size;
   __shared__ float froom[THREADS > 64 ? THREADS / 64 : 1];
   __shared__ unsigned uroom[THREADS > 64 ? THREADS / 64 : 1];
-  const long long r = (long long)blockIdx.x * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
+  const long long r = (a.first + blockIdx.x) * ROWS + (ROWS > 1 ? threadIdx.x / THREADS : 0);
   if (r >= a.rows) return;   // (whole waves: rows share a workgroup only where a wave has one)
   const int t = threadIdx.x % THREADS;
   auto add = [](float x, float y) { return x + y; };
@@ -245,13 +245,13 @@ __global__ __launch_bounds__(THREADS == 64 ? 256 : THREADS) void k_norm(NormArgs
 }
 
 template <int TYPE, bool S8, int THREADS, int V>
-hipError_t run(const NormArgs &a, hipStream_t s)
+hipError_t run(NormArgs a, hipStream_t s)
 {
-  constexpr int rows = THREADS == 64 ? 4 : 1;
-  const long long blocks = (a.rows + rows - 1) / rows;
-  if (blocks >= 1ll << 31) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((k_norm<TYPE, S8, THREADS, V>), dim3((unsigned)blocks), dim3(THREADS == 64 ? 256 : THREADS), 0, s, a);
-  return hipGetLastError();
+  constexpr int rows = THREADS == 64 ? 4 : 1, threads = THREADS == 64 ? 256 : THREADS;
+  return launch_pieces((a.rows + rows - 1) / rows, threads, [&](long long first, unsigned count) {
+    a.first = first;
+    hipLaunchKernelGGL((k_norm<TYPE, S8, THREADS, V>), dim3(count), dim3(threads), 0, s, a);
+  });
 }
 
 // Eight columns a thread as long as a workgroup has the threads, whatever the rows: bf16, us, against four times as many columns

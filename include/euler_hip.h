@@ -319,7 +319,7 @@ typedef struct ehip_route_args {
 
 typedef struct ehip_route ehip_route_t;
 
-/* experts up to 1024, topk up to 32, groups up to 64, tokens * topk below 2^30. */
+/* experts up to 1024, topk up to 32, groups up to 64, tokens * topk below 2^30, tokens up to 2^29 - 128. */
 EHIP_API int ehip_route_create(const ehip_route_desc_t *desc, ehip_route_t **out);
 EHIP_API int ehip_route_destroy(ehip_route_t *route);
 /* int32 values of a plan for so many tokens (offsets, slots, and what the call keeps while it runs); -1 = bad argument */

@@ -211,3 +211,12 @@ def test_stream_and_graph():
         c.y.copy_(torch.randn_like(c.y))
         g.replay()
         c.check()
+
+
+def test_more_rows_than_a_launch_has_threads():
+    """64 threads a row: 2^26 rows and more go out in two launches"""
+    m = (1 << 26) + 70
+    x = torch.empty(m, dtype=torch.bfloat16, device="cuda").random_(1, 200)
+    out = torch.zeros_like(x)
+    E.Norm(E.make_norm_desc(1, pre=E.NORM_NONE, block_scale=0.5)).execute(out, x, m)
+    assert torch.equal(out, x * 0.5)

@@ -100,3 +100,14 @@ def test_scales_without_codes_are_refused(kind):
     for rows in (0, 4):
         with pytest.raises(E.EulerHipError, match="s8 rows"):
             h.execute(256, 256, rows, output_scale=256)
+
+
+def test_route_counts_tokens_that_a_launch_can_have():
+    """8 threads a token, and a launch's are counted in 32 bits"""
+    h = E.Router(E.make_route_desc(2, 1))
+    assert h.plan_ints((1 << 29) - 128) > 0
+    for tokens in ((1 << 29) - 127, (1 << 30) - 1):
+        with pytest.raises(ValueError):
+            h.plan_ints(tokens)
+        with pytest.raises(E.EulerHipError, match="tokens"):
+            h.execute(256, 256, 256, 256, tokens)
