@@ -186,25 +186,51 @@ template <> struct Product<EHIP_S8> {
   __device__ static __forceinline__ Acc mma(i4 w, i4 x, Acc c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(w, x, c, 0, 0, 0); }
 };
 
-// The activation functions in single precision.
-// GELU: v * Phi(v) = max(v, 0) - |v| / 2 * erfc(|v| / sqrt(2)).  With x = |v| / 2 the second term is x * 2^p(x), p fitted to
-// log2(erfc(sqrt(2) x)) on 0 <= x <= 3 (degree 8, p(0) = 0; least squares of the term itself, weighted until its largest error is
-// even): off by at most 4.3e-8, and by 8.4e-8 of |v|, in single precision.  Past 3 the term is below 6e-9.  One transcendental
-// instruction and 12 others, where the library's error function takes dozens: s8 3001 x 4104 x 5000 99 -> 85 us.
-// SiLU: the exponential of a large negative v is infinite and the result -0, as the limit is.
-template <int ACT>
+// The activation functions in single precision, for results of type TYPE.  Units are 2^-24 of a value.
+// GELU: v * Phi(v) = max(v, 0) - |v| * Phi(-|v|) = max(v, 0) - x * erfc(sqrt(2) x), x = |v| / 2.  For v < 0 the second term is all of
+// the result, and a gate's partner can make it large: it keeps its digits however small it is, down to the least exponential, whose
+// place is v = -13.
+//   16-bit results: x * 2^(x p(x)), p of degree 10 fitted to log2(erfc(sqrt(2) x)) / x on 0 <= x <= 6.6 (least squares of the term,
+//   weighted until its largest error, against 2 units of |v| or 5e-5 of the term, is even): off by at most 3.3 units of |v|, and
+//   by 8.2e-5 of the term down to v = -8, 1.3e-4 from there (f16 rounds by 4.9e-4); the exponent's roundings add 14 (1 + v^2) units
+//   of the term.  One transcendental instruction and 15 others.
+//   f32 results: x * exp(-2 x^2) * E(x), E = erfc(sqrt(2) x) exp(2 x^2): 1 at 0 and like 1 / x far out, so a polynomial without a
+//   constant in t = 1 / (1 + 0.7 x).  Degree 9 on 0 <= x <= 7, fitted likewise: 3.2e-8.  With the roundings (of t, counted 2.3
+//   times, and of the exponent, v^2 / 2 times) 16 + 2 v^2 units of the term.  Two transcendental instructions and 17 others: f16 results
+//   of s8 3001 x 4104 x 5000 would take 80 us with it where they take 77, f32 results of bf16 4096 x 1024 x 4096 take 43 (41 without).
+// SiLU: off by at most 8 + 2 |v| units (the exponent's roundings); the exponential of a large negative v is infinite and the
+// result -0, as the limit is.
+template <int ACT, int TYPE>
 __device__ __forceinline__ float activate(float v)
 {
   if (ACT == EHIP_ACT_RELU) return v > 0.0f ? v : v != v ? v : 0.0f;
   if (ACT == EHIP_ACT_GELU) {
-    const float h = 0.5f * v, x = __builtin_fminf(__builtin_fabsf(h), 3.0f);
-    float p = __builtin_fmaf(x, -0.00048698447f, 0.0035916152f);
-    p = __builtin_fmaf(x, p, -0.0084150452f);
-    p = __builtin_fmaf(x, p, -0.0087055275f);
-    p = __builtin_fmaf(x, p, 0.11592617f);
-    p = __builtin_fmaf(x, p, -0.42102069f);
-    p = __builtin_fmaf(x, p, -1.8366486f);
-    p = __builtin_fmaf(x, p, -2.3022220f);
+    const float h = 0.5f * v;
+    if (TYPE == EHIP_F32) {
+      const float x = __builtin_fminf(__builtin_fabsf(h), 7.0f);
+      const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(x, 0.7f, 1.0f));
+      float p = __builtin_fmaf(t, -0.058291804f, 0.28794315f);
+      p = __builtin_fmaf(t, p, -0.51142806f);
+      p = __builtin_fmaf(t, p, 0.31834787f);
+      p = __builtin_fmaf(t, p, -0.046219379f);
+      p = __builtin_fmaf(t, p, 0.21101590f);
+      p = __builtin_fmaf(t, p, 0.23966576f);
+      p = __builtin_fmaf(t, p, 0.27972373f);
+      p = __builtin_fmaf(t, p, 0.27924281f);
+      const float e = __builtin_amdgcn_exp2f(x * (x * -2.8853901f));
+      return __builtin_fmaf(-(x * e), p * t, h + __builtin_fabsf(h));
+    }
+    const float x = __builtin_fminf(__builtin_fabsf(h), 6.6f);
+    float p = __builtin_fmaf(x, 1.3627697e-7f, -4.6344026e-6f);
+    p = __builtin_fmaf(x, p, 6.6200366e-5f);
+    p = __builtin_fmaf(x, p, -5.0509541e-4f);
+    p = __builtin_fmaf(x, p, 0.0020654162f);
+    p = __builtin_fmaf(x, p, -0.0026251888f);
+    p = __builtin_fmaf(x, p, -0.017977515f);
+    p = __builtin_fmaf(x, p, 0.12327838f);
+    p = __builtin_fmaf(x, p, -0.42386577f);
+    p = __builtin_fmaf(x, p, -1.8361757f);
+    p = __builtin_fmaf(x, p, -2.3022454f);
     return __builtin_fmaf(-x, __builtin_amdgcn_exp2f(x * p), h + __builtin_fabsf(h));
   }
   if (ACT == EHIP_ACT_SILU) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * v));

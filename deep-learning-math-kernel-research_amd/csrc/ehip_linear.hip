@@ -195,13 +195,13 @@ __global__ __launch_bounds__(512) void k_linear_split(LinearArgs a)
         const f4 gate = finish_sums(a, total(2 * n, m), at, xs);
         const f4 up = finish_sums(a, total(NT > 1 ? 2 * n + 1 : 0, m), at + 16, xs);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = activate<act.value>(gate[r]) * up[r];
+        for (int r = 0; r < 4; ++r) v[r] = activate<act.value, type.value>(gate[r]) * up[r];
         col = (tile >> 2) * 32 + g * 8 + ((tile & 3) >> 1) * 4;
       } else {
         const int tile = tile0 + n;
         const f4 t = finish_sums(a, total(n, m), ((long long)blk.expert * a.tiles + tile) * 16 + g * 4, xs);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = activate<act.value>(t[r]);
+        for (int r = 0; r < 4; ++r) v[r] = activate<act.value, type.value>(t[r]);
         col = (tile >> 2) * 64 + g * 16 + (tile & 3) * 4;
       }
       store_columns<type.value, 4>(v, a.out + row.out * a.ldo + (long long)col * SIZE,

@@ -221,7 +221,7 @@ __global__ __launch_bounds__(WN * WM * 64) void k_linear_tile(LinearArgs a)
           }
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          v[0][j] = activate<act.value>(v[0][j]);
+          v[0][j] = activate<act.value, type.value>(v[0][j]);
           if (GATED) v[0][j] *= v[GATED][j];
         }
         if (early) {

@@ -353,3 +353,50 @@ def test_more_weights_than_a_launch_has_threads():
     for i, e in enumerate((0, 30, 31)):
         assert torch.equal(out[i], w[e] * x[i])
     h.close()
+
+
+def act_alone(d, kind, otype):
+    """(value, error) of an activation by itself, relative to the value also where that is tiny.  Units are 2^-24.
+    GELU max(v, 0) - t: f32 results, t off by 16 + 2 v^2 units of itself (fit 1, Horner's last steps 2, t's argument and its reciprocal
+    3, counted 2.3 times, the exponential 2, products 3; the exponent 2.5, v^2 / 2 times); 16-bit results, by the fit's 1.3e-4 of
+    itself and no more than 3.3 units of |v|, and by 14 (1 + v^2) units (the partial sums of the exponent's polynomial, carried on,
+    and the exponential's 2); one subtraction.
+    SiLU: 8 + 2 |v| units (the exponential 2, a sum, its reciprocal 2, a product; the exponent 1.5, |v| times).
+    Exponentials and reciprocals below 2^-126 are 0."""
+    u, least = ref.EPS32, 2.0 ** -125 * d.abs().clamp(max=100)
+    if kind == E.ACT_GELU:
+        t = 0.5 * d.abs() * torch.erfc(d.abs() * math.sqrt(0.5))
+        want = d.clamp(min=0) - t
+        own = (16 + 2 * d * d) * u * t if otype == E.F32 else torch.minimum(1.3e-4 * t, 3.3 * u * d.abs()) + (2 + 14 * (1 + d * d)) * u * t
+        return want, own + 2 * u * want.abs() + least
+    if kind == E.ACT_SILU:
+        want = d * torch.sigmoid(d)
+        return want, (8 + 2 * d.abs()) * u * want.abs() + least
+    return (d.clamp(min=0) if kind == E.ACT_RELU else d), torch.zeros_like(d)
+
+
+@pytest.mark.parametrize("form", [1, 5, 7, 8])
+@pytest.mark.parametrize("otype", [E.F32, E.F16, E.BF16])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("activation", [E.ACT_NONE, E.ACT_RELU, E.ACT_GELU, E.ACT_SILU])
+def test_activations_keep_their_digits(activation, gated, otype, form, monkeypatch):
+    """the function by itself, on biases: an output a value; gated, with partners that lift tiny values to about 1"""
+    monkeypatch.setenv("EHIP_LINEAR_FORM", str(form))
+    v = torch.cat([torch.linspace(-16, 16, 20011), torch.linspace(-60, 60, 2001), torch.linspace(-0.3, 0.3, 3001), torch.logspace(-30, 0, 400),
+                   -torch.logspace(-30, 0, 400), torch.tensor([0.0, -100.0, 1e30, -1e30, 3e38, -3e38])]).cuda()
+    n = len(v)
+    want, off = act_alone(v.double(), activation, otype)
+    bias = v
+    if gated:
+        partner = torch.where(want.abs() > 1e-34, 1 / want, torch.ones_like(want)).clamp(-1e35, 1e35).float()
+        bias = torch.cat([v, partner])
+        want, off = want * partner.double(), off * partner.double().abs() + 2 * ref.EPS32 * (want * partner.double()).abs()
+    h = E.Linear(E.make_linear_desc(1, n, output_type=otype, activation=activation, gated=gated, with_bias=True))
+    h.prepare(torch.ones((len(bias), 1), dtype=torch.bfloat16, device="cuda"), bias=bias)
+    x, out = torch.zeros((3, 1), dtype=torch.bfloat16, device="cuda"), torch.full((3, n), math.nan, dtype=TORCH[otype], device="cuda")
+    h.execute(out, x, 3)
+    torch.cuda.synchronize()
+    # (past the largest f16 values are infinite)
+    fits = want.abs() < (65504 if otype == E.F16 else 3e38)
+    for row in out:
+        ref.close(row[fits], want[fits], off[fits])
