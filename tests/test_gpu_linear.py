@@ -400,3 +400,90 @@ def test_activations_keep_their_digits(activation, gated, otype, form, monkeypat
     fits = want.abs() < (65504 if otype == E.F16 else 3e38)
     for row in out:
         ref.close(row[fits], want[fits], off[fits])
+
+
+def exact_rows(g, *shape, dtype=torch.bfloat16):
+    """small whole numbers: every sum of their products is exact in f32 and s32, in any order"""
+    return torch.randint(-4, 5, shape, generator=g, device="cuda").to(dtype)
+
+
+# Runs of 128-byte steps of K for each of eight waves: the loops of every form in several turns with every remainder; waves with
+# fewer steps than others, with none; a part of a step behind the last
+@pytest.mark.parametrize("form", range(9))
+@pytest.mark.parametrize("itype", TYPES)
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("steps, tail", [(33, 0), (40, 5), (41, 0), (48, 16), (50, 1), (56, 0), (61, 8), (64, 63), (72, 3), (77, 0)])
+def test_every_step_of_a_long_sum_counts_once(steps, tail, gated, itype, form, monkeypatch):
+    """bit for bit: a step that is dropped, repeated or taken from another's registers cannot hide in a bound"""
+    monkeypatch.setenv("EHIP_LINEAR_FORM", str(form))
+    g = torch.Generator(device="cuda")
+    g.manual_seed(steps * 100 + tail)
+    ic, m, oc = steps * (128 if itype == E.S8 else 64) + tail, 37, 70
+    n2 = 2 * oc if gated else oc
+    x, w = exact_rows(g, m, ic, dtype=TORCH[itype]), exact_rows(g, n2, ic, dtype=TORCH[itype])
+    ones = torch.ones(max(m, n2), device="cuda") if itype == E.S8 else None
+    h = E.Linear(E.make_linear_desc(ic, oc, input_type=itype, output_type=E.F32, gated=gated))
+    h.prepare(w, scale=ones)
+    out = torch.full((m, oc), math.nan, device="cuda")
+    h.execute(out, x, m, input_scale=ones)
+    a = x.double() @ w.double().t().contiguous()
+    want = a[:, :oc] * a[:, oc:] if gated else a
+    assert torch.equal(out, want.float())
+
+
+@pytest.mark.parametrize("form", range(9))
+@pytest.mark.parametrize("itype", TYPES)
+@pytest.mark.parametrize("steps, tail", [(36, 0), (45, 7), (70, 0)])
+def test_every_step_of_the_experts_long_sums_counts_once(steps, tail, itype, form, monkeypatch):
+    monkeypatch.setenv("EHIP_LINEAR_FORM", str(form))
+    g = torch.Generator()
+    g.manual_seed(steps)
+    tokens, experts, topk, oc = 60, 5, 2, 70
+    slots, offsets, ids = plan(g, tokens, experts, topk, empty=(3,))
+    g = torch.Generator(device="cuda")
+    g.manual_seed(steps)
+    ic = steps * (128 if itype == E.S8 else 64) + tail
+    for gated in (True, False):
+        n2 = 2 * oc if gated else oc
+        x, w = exact_rows(g, tokens, ic, dtype=TORCH[itype]), exact_rows(g, experts, n2, ic, dtype=TORCH[itype])
+        ones = torch.ones(max(tokens, experts * n2), device="cuda") if itype == E.S8 else None
+        h = E.Linear(E.make_linear_desc(ic, oc, experts, itype, E.F32, gated=gated))
+        h.prepare(w, scale=ones)
+        out = torch.full((tokens * topk, oc), -7.0, device="cuda")
+        h.execute_experts(out, x, slots, offsets, tokens * topk, topk, input_scale=ones, input_rows=E.ROWS_TOKEN, output_rows=E.ROWS_SLOT)
+        for s, e in enumerate(ids.tolist()):
+            if e < 0:
+                assert (out[s] == -7).all()
+        live = (ids >= 0).cuda()
+        at = ids.clamp(min=0).cuda()
+        a = torch.zeros((tokens * topk, n2), dtype=torch.float64, device="cuda")
+        for e in range(experts):
+            here = live & (at == e)
+            a[here] = x[torch.arange(tokens * topk, device="cuda")[here] // topk].double() @ w[e].double().t().contiguous()
+        want = a[:, :oc] * a[:, oc:] if gated else a
+        assert torch.equal(out[live], want[live].float())
+
+
+@pytest.mark.parametrize("itype, m, ic, oc", [(E.BF16, 1, 4096, 4096), (E.F16, 64, 2048, 1000), (E.S8, 16, 4096, 4096), (E.BF16, 1024, 4096, 1000),
+                                              (E.S8, 1500, 4104, 1000), (E.F16, 2100, 4096, 2048)])
+def test_products_of_a_models_size(itype, m, ic, oc):
+    """the forms that these sizes take, on whole numbers, bit for bit, and on ordinary values within single precision's error"""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m)
+    x, w = exact_rows(g, m, ic, dtype=TORCH[itype]), exact_rows(g, oc, ic, dtype=TORCH[itype])
+    ones = torch.ones(max(m, oc), device="cuda") if itype == E.S8 else None
+    h = E.Linear(E.make_linear_desc(ic, oc, input_type=itype, output_type=E.F32))
+    h.prepare(w, scale=ones)
+    out = torch.full((m, oc), math.nan, device="cuda")
+    h.execute(out, x, m, input_scale=ones)
+    assert torch.equal(out, (x.double() @ w.double().t().contiguous()).float())
+    c = Case(m, ic, oc, itype, E.F32, bias=True, residual=True)
+    c.run()
+    torch.cuda.synchronize()
+    if itype != E.S8:
+        # at most ic sums, each off by 2^-23 of a partial sum, which is within 6 of its deviation (the root of the products' squares);
+        # independent errors add by squares
+        want, _ = ref.linear(c.x, c.w, c.d, c.b, None, None, c.r)
+        size = ((c.x.double() ** 2) @ (c.w.double() ** 2).t().contiguous()).sqrt() + c.b.double().abs() + c.r.double().abs()
+        assert ((c.out.double() - want).abs() / size).max() <= 6 * 2 * ref.EPS32 * math.sqrt(ic)
+    c.check()
