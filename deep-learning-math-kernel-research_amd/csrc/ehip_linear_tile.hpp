@@ -6,7 +6,9 @@
 
 namespace ehip {
 
-// 64 lanes x 16 bytes from memory into LDS at lds + 16 * lane, no registers between.  The wait is the caller's.
+// 64 lanes x 16 bytes from memory into LDS at lds + 16 * lane, no registers between.  The wait is the caller's, and so is the order:
+// every wave's reads of a place end before the meeting that the loads into it follow, reads of what they bring come behind the
+// next one, and meet() lets no access to memory past it.  Nothing else in these kernels uses m0 (tests/test_compiled_kernels.py).
 __device__ __forceinline__ void load_to_lds(const char *src, unsigned lds)
 {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" : : "s"(lds), "v"(src) : "m0");
