@@ -63,12 +63,13 @@ hipError_t launch_linear_constants(float *dst, const float *src, int experts, in
 
 // ---- few rows ----------------------------------------------------------------------------------------------------
 // A workgroup has NT tiles of 16 weights rows x MT tiles of 16 activations rows; its waves share K out in runs of steps of 128
-// bytes, so no weight is read twice and they stream past as runs of KBs, straight into registers, P steps ahead.  Activations
+// bytes, so a workgroup reads no weight twice and they stream past as runs of KBs, straight into registers, P steps ahead.  Activations
 // come by whole lines, 8 lanes a row, and change lanes through a corner of LDS that is the wave's own (a load that gave every
 // lane the 16 bytes that its matrix operand has would be 64 accesses instead of 16, and the loads bound these kernels).  The
 // waves' sums meet in LDS, in the order of the waves.
-// Measured: bf16 1 x 4096 x 4096 7.2 us, 4.6 TB/s of weights; s8 gated 16 x 4096 x 8192 12.2 us, 5.5 TB/s; f16 64 x 2048 x 1000
-// 3.9 us; 64 slots of 32 experts of 2048 x 2816 57 us, 5.7 TB/s.  Weights' bytes bound it up to some 16 rows, then the loads:
+// Measured, weights out of memory (out of the memory-side cache): bf16 1 x 4096 x 4096 8.4 us, 4.0 TB/s of weights (5.2 us); s8 gated
+// 16 x 4096 x 8192 15.4 us, 4.4 TB/s (12.3); 64 slots of 32 experts of 2048 x 2816 57 us, 5.7 TB/s (51); f16 64 x 2048 x 1000 (4.0).
+// Weights' bytes bound it up to some 16 rows, then the loads:
 // 64 x 64 results of 64 steps take a CU 11 us, twice what their products do.
 template <int TYPE, int NT, int MT, int P>
 __global__ __launch_bounds__(512) void k_linear_split(LinearArgs a)
@@ -236,9 +237,10 @@ enum Form { SPLIT_1X1, SPLIT_2X1, SPLIT_4X1, SPLIT_2X2, SPLIT_4X2, SPLIT_4X4, TI
 
 // What a form takes, in us, from what it measured on an idle card (bf16, f16 and s8 alike: a step is 128 bytes of K, and so are
 // its loads and its matrix instructions).  All forms: no faster than the bytes at 5.2 TB/s; what is hidden behind those is
-// not hidden whole.  Sweeps of 1 - 4096 rows, K 512 -
-// 8192 bytes, 1024 - 8192 columns, and of experts with 1 - 770 rows each: the form with the least sum is the fastest one or
-// within 15 % of it, in the worst case found 30 % (20 rows, 4096 x 4096: 9.8 us for 8.0).
+// not hidden whole.  Sweeps of 1 - 4096 rows, K 512 - 8192 bytes, 1024 - 8192 columns, and of experts with 1 - 770 rows each: the
+// form with the least sum is the fastest one or within 15 % of it, in the worst case found 27 % (256 rows, bf16 512 -> 1024: 5.2 us
+// for 4.1).  What it does not know: that each block of rows reads the weights again (32 rows, bf16 4096 x 4096: 9.7 for
+// 7.8), and that rows at addresses that are no multiple of 16 bytes are slower to load (s8 1024 x 4097 x 2000: 39 for 31).
 struct FormCost {
   int nt, mt;          // tiles of a workgroup's results
   int resident;        // workgroups of a CU

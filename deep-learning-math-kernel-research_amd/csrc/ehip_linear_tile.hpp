@@ -17,8 +17,8 @@ __device__ __forceinline__ void load_to_lds(const char *src, unsigned lds)
 // A workgroup has WN x WM waves of NTW x MTW tiles of 16 x 16 results.  A step is 128 bytes of K, in two halves.  A wave multiplies one half out of registers while it reads the next into others.  The workgroup meets once a step,
 // between the halves: by then every wave has read the whole step, and the next one has arrived; another one is loaded into the
 // place that came free.  LDS holds STAGES steps.
-// Measured: bf16 gated 4096 x 4096 x 8192 418 - 453 us (1213 - 1316 TFLOP/s; the products alone 357 us, at the clock that they
-// leave), of which the results are 40 us and loads that miss L2 another 40; s8 4096 x 4096 x 4096 58 us (2370 TOPS).
+// Measured: bf16 gated 4096 x 4096 x 8192 382 - 411 us (1338 - 1439 TFLOP/s; by card and clock: other boxes took up to 453), of which
+// the results are 40 us and loads that miss L2 another 40; s8 4096 x 4096 x 4096 58 us (2370 TOPS).
 // ALIGNED: rows of activations at multiples of 16 bytes and a whole number of 16-byte parts in K, so they go straight into LDS
 // like the weights; else through registers.
 template <int TYPE, int NTW, int MTW, int WN, int WM, int STAGES, bool ALIGNED>
