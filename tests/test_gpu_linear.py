@@ -320,6 +320,41 @@ def test_the_name_is_of_the_kernel_that_runs(m, ic, oc, otype, residual, gated, 
         assert name != "k_linear_tile<128x128, deep>"
 
 
+def test_the_name_counts_the_outputs_bytes():
+    """f32 results and their residual are four times the bytes of bf16 ones: another form is the faster one"""
+    names = [E.Linear(E.make_linear_desc(256, 512, output_type=t, with_residual=r)).kernel_name(2048) for t, r in ((E.BF16, False), (E.F32, True))]
+    assert names == ["k_linear_split<4x4>", "k_linear_tile<128x128, deep>"]
+
+
+@pytest.mark.parametrize("form, m", [(5, (1 << 29) + 70), (6, (1 << 31) - 1), (8, (1 << 31) - 1)])
+def test_more_rows_than_a_launch_has_threads(form, m, monkeypatch):
+    """a launch's threads are counted in 32 bits: more workgroups than that go out in several"""
+    monkeypatch.setenv("EHIP_LINEAR_FORM", str(form))
+    h = E.Linear(E.make_linear_desc(1, 1))
+    h.prepare(torch.full((1,), 0.5, dtype=torch.bfloat16, device="cuda"))
+    x = torch.empty(m, dtype=torch.bfloat16, device="cuda").random_(1, 200)
+    out = torch.zeros_like(x)
+    h.execute(out, x, m)
+    assert torch.equal(out, x * 0.5)
+
+
+def test_more_weights_than_a_launch_has_threads():
+    """64 GiB of packed weights: a thread packs 16 bytes of them"""
+    experts, oc = 32, 1 << 24
+    w = torch.empty((experts, oc), dtype=torch.bfloat16, device="cuda").random_(1, 200)
+    h = E.Linear(E.make_linear_desc(1, oc, experts=experts))
+    h.prepare(w)
+    x = torch.tensor([[0.5], [2.0], [1.0]], dtype=torch.bfloat16, device="cuda")
+    out = torch.zeros((3, oc), dtype=torch.bfloat16, device="cuda")
+    slots = torch.arange(3, dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([0] + [1] * 30 + [2, 3], dtype=torch.int32, device="cuda")   # experts 0, 30 and 31
+    h.execute_experts(out, x, slots, offsets, 3, 1)
+    torch.cuda.synchronize()
+    for i, e in enumerate((0, 30, 31)):
+        assert torch.equal(out[i], w[e] * x[i])
+    h.close()
+
+
 def act_alone(d, kind, otype):
     """(value, error) of an activation by itself, relative to the value also where that is tiny.  Units are 2^-24.
     GELU max(v, 0) - t: f32 results, t off by 16 + 2 v^2 units of itself (fit 1, Horner's last steps 2, t's argument and its reciprocal
