@@ -320,12 +320,6 @@ def test_the_name_is_of_the_kernel_that_runs(m, ic, oc, otype, residual, gated, 
         assert name != "k_linear_tile<128x128, deep>"
 
 
-def test_the_name_counts_the_outputs_bytes():
-    """f32 results and their residual are four times the bytes of bf16 ones: another form is the faster one"""
-    names = [E.Linear(E.make_linear_desc(256, 512, output_type=t, with_residual=r)).kernel_name(2048) for t, r in ((E.BF16, False), (E.F32, True))]
-    assert names == ["k_linear_split<4x4>", "k_linear_tile<128x128, deep>"]
-
-
 @pytest.mark.parametrize("form, m", [(5, (1 << 29) + 70), (6, (1 << 31) - 1), (8, (1 << 31) - 1)])
 def test_more_rows_than_a_launch_has_threads(form, m, monkeypatch):
     """a launch's threads are counted in 32 bits: more workgroups than that go out in several"""
